@@ -2,7 +2,9 @@
 
 One compiler line per library (run in parallel): ``hipcc`` for the gfx950
 kernels — ``libptcell.so`` (InT / hGRU cell, include/pt_cell.h) and
-``libptlstm.so`` (ConvLSTM cell, include/pt_lstm.h) — and ``g++`` for the host
+``libptlstm.so`` (ConvLSTM cell, include/pt_lstm.h), ``libptscan.so`` (gated
+linear recurrences, include/pt_scan.h), ``libptclip.so`` (gradient norm and
+clipping, include/pt_clip.h) — and ``g++`` for the host
 TFRecord reader ``libpttfr.so`` (include/pt_tfrecord.h, zlib).  They sit next
 to the ctypes bindings so they travel with the repository snapshot to the GPU
 box.  ``libptcell_diag.so`` is the same cell library built with -DPT_DIAG=1
@@ -33,12 +35,17 @@ _CELL = ([os.path.join(CSRC, "pt_cell.hip"), os.path.join(CSRC, "pt_readout.hip"
 _LSTM = ([os.path.join(CSRC, "pt_lstm.hip")],
          [os.path.join(CSRC, "pt_device.h"), os.path.join(CSRC, "pt_graph.h"),
           os.path.join(INC, "pt_lstm.h")])
+# no packed-FP32 instructions at all (HIP_FLAGS' -fno-slp-vectorize keeps one
+# source of them out; this, every other)
+_NO_PK = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 LIBS = {
     "libptcell.so": _CELL,
     "libptcell_diag.so": _CELL + (["-DPT_DIAG=1"],),
     "libpttfr.so": ([os.path.join(CSRC, "pt_tfrecord.cpp")], [os.path.join(INC, "pt_tfrecord.h")]),
     "libptlstm.so": _LSTM,
     "libptlstm_diag.so": _LSTM + (["-DPT_DIAG=1"],),
+    "libptscan.so": ([os.path.join(CSRC, "pt_scan.hip")], [os.path.join(INC, "pt_scan.h")], _NO_PK),
+    "libptclip.so": ([os.path.join(CSRC, "pt_clip.hip")], [os.path.join(INC, "pt_clip.h")], _NO_PK),
 }
 OUT = os.path.join(HERE, "libptcell.so")      # kept for callers of the old single-library API
 # The compiler line of the HIP libraries; part of the source stamp.
