@@ -42,11 +42,13 @@ typedef struct pt_scan_desc {
     int32_t dtype;      /* of x, y and their gradients                           */
     int64_t batch;      /* B >= 1                                                */
     int64_t channels;   /* C >= 1                                                */
-    int64_t steps;      /* T >= 1                                                */
-    int64_t inner;      /* N >= 1                                                */
+    int64_t steps;      /* T, 1 to 2^30                                          */
+    int64_t inner;      /* N, 1 to 2^29 - 1                                      */
 } pt_scan_desc;
 
-/* One sequence tensor: element strides over batch, channel and step. */
+/* One sequence tensor: element strides over batch, channel and step.  The gates
+ * of a call share theirs (as slices of one tensor do), and so do their
+ * gradients; x, y and dx may differ from each other. */
 typedef struct pt_scan_view {
     void* data;
     int64_t sb, sc, st;

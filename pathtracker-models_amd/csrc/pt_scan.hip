@@ -11,8 +11,10 @@
 // chunk's start.  a is a logistic value, 0 <= a <= 1, so products can only
 // underflow, never overflow.
 //
-// Layout.  A lane owns V neighbouring columns (channel, inner), so every load
-// of a wave is 64 V neighbouring elements of one step.  Where the columns do
+// Layout.  A lane owns a column (channel, inner), so every load of a wave is 64
+// neighbouring elements of one step.  Two 16-bit columns a lane would halve the
+// loads, but what a step keeps until its gradient is known then passes 128
+// registers: the backward spilled and took 3.1 times as long.  Where the columns do
 // not fill the card the time axis is also cut over workgroups (`segs`): a
 // first launch reduces each segment to (P, q), and the second starts each
 // segment from the composition of those before it.
@@ -20,6 +22,8 @@
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
+
+#include <algorithm>
 
 #include "pt_scan.h"
 
@@ -36,16 +40,19 @@ int fail(int code, const char* msg) {
   return code;
 }
 
-constexpr int64_t MAX_SEGS = 64;
-constexpr int SPLIT_W = 16;      // waves of a workgroup when the time axis is cut over workgroups
+constexpr int MAX_SEGS = 64;
+constexpr int SPLIT_W = 8;       // waves of a workgroup when the time axis is cut over workgroups
 
-struct View {
-  char* p;
-  int64_t sb, sc, st;      // element strides
+// One kind of sequence tensor (all gates share their strides): strides in bytes.
+struct Strides {
+  int64_t b, c, t;
 };
 
 struct Args {
-  View x[4], y, dx[4];     // y: the output, or dy in the backward
+  const char* x[4];        // the gates
+  char* dx[4];             // their gradients
+  char* y;                 // the output, or dy in the backward
+  Strides xs, ds, ys;
   const float* h0;
   const int64_t* len;
   float* h_last;
@@ -53,13 +60,14 @@ struct Args {
   const float* d_h_last;
   const float* d_c_last;
   float* d_h0;
-  float* saved;            // [chunk][B][C N]: the state before a chunk (chunk 0: h0)
+  float* saved;            // [chunk of the backward][B][C N]: the state before it (the first: h0)
   float* agg;              // [segment][B][C N] pairs (P, q)
-  int64_t T, cols_all;     // steps; B C N
+  int64_t cols_all;        // B C N
   int64_t C, N;
   int64_t cg, groups;      // channels per column group, groups per batch row
   int64_t outer;           // B groups
-  int64_t seg_steps;       // a multiple of the chunk
+  int T;                   // steps
+  int seg_steps;           // a multiple of the chunk
   int tiles, segs;
 };
 
@@ -87,12 +95,13 @@ template <bool ACC> __device__ __forceinline__ float recip(float d) {
   return r;
 }
 
-// s(x) and s(-x), both to full relative accuracy (1 - s(x) would cancel).
-template <bool ACC> __device__ __forceinline__ void logistic(float x, float& s, float& sm) {
+// s(x), s(-x) and their product, each to full relative accuracy (1 - s would
+// cancel).  What a caller does not use costs nothing.
+struct Logistic { float s, sm, p; };
+template <bool ACC> __device__ __forceinline__ Logistic logistic(float x) {
   const float e = exp_minus<ACC>(__builtin_fabsf(x));
   const float big = recip<ACC>(1.f + e), small = e * big;
-  s = x >= 0.f ? big : small;
-  sm = x >= 0.f ? small : big;
+  return {x >= 0.f ? big : small, x >= 0.f ? small : big, small * big};
 }
 
 // tanh(x) and its derivative 4 e / (1 + e)^2, e = exp(-2|x|).  f32 data: the
@@ -122,12 +131,35 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Where a workgroup works: column tile, row, segment; and a lane's columns.
-template <int V> struct Where {
-  int seg, lane, wave;
-  int64_t b, row, end;       // batch row; its end; index of the group's first channel in [B C]
-  bool on;                   // this lane's columns exist
-  int64_t state;             // index of this lane's first column in [B][C][N]
+// A global address that every lane of the wave holds alike, kept in scalar
+// registers: a step's address is then a scalar plus one 32-bit lane offset for
+// all steps.  (Left to itself the compiler keeps a 64-bit vector pointer each.)
+using gptr = __attribute__((address_space(1))) char*;
+__device__ __forceinline__ gptr scalar(const char* p) {
+  uint64_t u = (uint64_t)p;
+  asm("" : "+s"(u));
+  return (gptr)u;
+}
+// A lane's 32-bit offset, seen by the compiler as one where it is used (hoisted
+// out of the loop as a 64-bit value it would no longer fold into the access).
+__device__ __forceinline__ uint32_t offset32(uint32_t off) {
+  asm("" : "+v"(off));
+  return off;
+}
+// The same for a scalar: what depends on it is computed where it is used (16
+// lane masks kept over the loop would be more than the scalar registers hold).
+__device__ __forceinline__ int here(int k) {
+  asm("" : "+s"(k));
+  return k;
+}
+template <typename T> using gval = __attribute__((address_space(1))) T;
+
+// Where a workgroup works: column tile, row, segment; and a lane's column.
+struct Where {
+  int seg, lane, wave, end;  // `end`: the batch row's
+  int64_t b, c0;             // batch row; the group's first channel
+  bool on;                   // this lane's column exists
+  int64_t state;             // this lane's column in [B][C][N]
   uint32_t off_c, off_n;     // channel in the group, position in the inner axis
 
   __device__ __forceinline__ Where(const Args& a) {
@@ -139,492 +171,451 @@ template <int V> struct Where {
     const uint32_t o = id % (uint32_t)a.outer;
     seg = (int)(id / (uint32_t)a.outer);
     const uint32_t br = o / (uint32_t)a.groups;
-    const int64_t g = o - br * (uint32_t)a.groups;
     b = br;
-    row = b * a.C + g * a.cg;
+    c0 = (int64_t)(o - br * (uint32_t)a.groups) * a.cg;
     const uint32_t cols = (uint32_t)(a.cg * a.N);
-    uint32_t j = tile * 64 * V + lane * V;
+    uint32_t j = tile * 64 + lane;
     on = j < cols;
     j = on ? j : 0;          // an idle lane reads column 0 and stores nothing
     off_c = a.cg == 1 ? 0 : j / (uint32_t)a.N;
     off_n = j - off_c * (uint32_t)a.N;
-    state = row * a.N + j;
+    state = (b * a.C + c0) * a.N + j;
     end = a.T;
     if (a.len) {
       const int64_t n = a.len[b];
-      end = n < 0 ? 0 : n < a.T ? n : a.T;
+      end = n < 0 ? 0 : n < a.T ? (int)n : a.T;
     }
   }
-  // byte offset of this lane within a step of the view (fits 32 bits: the host checks)
-  template <typename T> __device__ __forceinline__ uint32_t lane_off(const View& v) const {
-    return (uint32_t)((off_c * v.sc + off_n) * (int64_t)sizeof(T));
+  // byte offset of this lane within a step (fits 32 bits: the host checks)
+  __device__ __forceinline__ uint32_t lane_off(const Strides& s, int size) const {
+    return (uint32_t)(off_c * s.c) + off_n * (uint32_t)size;
   }
-  // the group's base at step 0
-  template <typename T> __device__ __forceinline__ char* base(const Args& a, const View& v) const {
-    const int64_t c0 = row - b * a.C;
-    return v.p + (b * v.sb + c0 * v.sc) * (int64_t)sizeof(T);
+  // byte offset of the group at step t
+  __device__ __forceinline__ int64_t base(const Strides& s, int t) const {
+    return b * s.b + c0 * s.c + (int64_t)t * s.t;
   }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ vec<T, V> load(const char* base, uint32_t off) {
-  return *(const vec<T, V>*)(base + off);
-}
-template <typename T, int V>
-__device__ __forceinline__ void store(char* base, uint32_t off, vec<T, V> v) {
-  *(vec<T, V>*)(base + off) = v;
-}
-
-// L steps from t0 of one view; steps at or behind lim are not read.
-template <typename T, int V, int L>
-__device__ __forceinline__ void load_steps(vec<T, V> (&r)[L], const char* base, int64_t st_bytes, uint32_t off,
-                                           int64_t t0, int64_t lim) {
-  const char* p = base + t0 * st_bytes;
-  if (t0 + L <= lim) {
+// L steps from p on; of which `live` are read, the others 0.
+template <typename T, int L>
+__device__ __forceinline__ void load_steps(T (&r)[L], const char* p, int64_t st, uint32_t off, int live) {
+  if (live >= L) {
+    off = offset32(off);
 #pragma unroll
-    for (int l = 0; l < L; ++l) r[l] = load<T, V>(p + l * st_bytes, off);
+    for (int l = 0; l < L; ++l, p += st) r[l] = *(const gval<T>*)(scalar(p) + off);
   } else {
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
-      r[l] = 0;
-      if (t0 + l < lim) r[l] = load<T, V>(p + l * st_bytes, off);
+    for (int l = 0; l < L; ++l, p += st) {
+      r[l] = (T)0.f;
+      if (l < live) r[l] = *(const gval<T>*)(scalar(p) + offset32(off));
     }
+  }
+}
+
+// The same for stores: steps from `live` on are written as 0, from `room` on not at all.
+template <typename T, int L>
+__device__ __forceinline__ void store_steps(const T (&r)[L], char* p, int64_t st, uint32_t off, int live, int room) {
+  if (live >= L) {
+    off = offset32(off);
+#pragma unroll
+    for (int l = 0; l < L; ++l, p += st) *(gval<T>*)(scalar(p) + off) = r[l];
+  } else {
+#pragma unroll
+    for (int l = 0; l < L; ++l, p += st)
+      if (l < room) *(gval<T>*)(scalar(p) + offset32(off)) = l < live ? r[l] : (T)0.f;
   }
 }
 
 template <int FORM> constexpr int gates_of() { return FORM == PT_SCAN_LEAKY ? 2 : 4; }
-// steps of one wave in a chunk: as many as two sets of the gates fit in registers
-template <int FORM> constexpr int steps_of() { return FORM == PT_SCAN_LEAKY ? 8 : 4; }
+// Steps of one wave in a chunk of the backward, as many as stay in 128
+// registers; the forward keeps less per step and takes twice as many.
+template <int FORM> constexpr int back_steps() { return FORM == PT_SCAN_LEAKY ? 8 : 4; }
 
-// Compose the waves' (P, q) of one chunk: the state before this wave's steps
-// from the one before the chunk, which becomes the one after it.
-template <int W, int V>
-__device__ __forceinline__ void compose(const float (&pq)[W][V][2][64], int wave, int lane, float (&carry)[V],
-                                        float (&mine)[V]) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float c = carry[v];
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      mine[v] = k == wave ? c : mine[v];
-      c = __builtin_fmaf(pq[k][v][0][lane], c, pq[k][v][1][lane]);
-    }
-    carry[v] = c;
-  }
-}
+using f32x2 = vec<float, 2>;
 
 // The state before segment `seg`.
-template <int V>
-__device__ __forceinline__ void start_state(const Args& a, const Where<V>& w, float (&c)[V]) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) c[v] = a.h0 ? a.h0[w.state + v] : 0.f;
+__device__ __forceinline__ float start_state(const Args& a, const Where& w) {
+  float c = a.h0 ? a.h0[w.state] : 0.f;
+  const f32x2* p = (const f32x2*)a.agg + w.state;
   for (int s = 0; s < w.seg; ++s) {
-    const float* p = a.agg + 2 * (s * a.cols_all + w.state);
-#pragma unroll
-    for (int v = 0; v < V; ++v) c[v] = __builtin_fmaf(p[2 * v], c[v], p[2 * v + 1]);
+    const f32x2 e = p[s * a.cols_all];
+    c = __builtin_fmaf(e[0], c, e[1]);
+  }
+  return c;
+}
+
+// a and b of one element of the forward.
+template <int FORM, typename T>
+__device__ __forceinline__ void coefs(float g0, float g1, float g2, float& a, float& b) {
+  constexpr bool ACC = sizeof(T) == 4;
+  const Logistic l = logistic<ACC>(g0);
+  if constexpr (FORM == PT_SCAN_LEAKY) {
+    a = l.sm;
+    b = l.s * g1;
+  } else {
+    float d;
+    a = logistic<ACC>(g1).s;
+    b = l.s * tanh_d<ACC>(g2, d);
   }
 }
 
 // Forward.  AGG: reduce a segment to (P, q) only.
-template <int FORM, typename T, int V, int W, bool AGG>
-__global__ __launch_bounds__(64 * W) void k_scan_fwd(Args a) {
+template <int FORM, typename T, int W, bool AGG>
+__global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
   static_assert(W > 1 || !AGG, "one wave never splits the time axis over workgroups");
-  constexpr int G = gates_of<FORM>(), L = steps_of<FORM>(), CH = W * L;
-  constexpr bool ACC = sizeof(T) == 4;
+  constexpr int G = gates_of<FORM>(), L = 2 * back_steps<FORM>(), CH = W * L;
   constexpr int GA = FORM == PT_SCAN_LEAKY ? 2 : 3;      // the gates that make a and b
-  __shared__ float pq[2][W][V][2][64];   // two sets in turn, as in the backward
-  const Where<V> w(a);
-  const int64_t t_beg = w.seg * a.seg_steps;
-  const int64_t t_end = t_beg + a.seg_steps < a.T ? t_beg + a.seg_steps : a.T;
-  const int64_t lim = w.end < t_end ? w.end : t_end;
-  const bool seq = !AGG && a.y.p != nullptr;
+  constexpr bool ACC = sizeof(T) == 4;
+  // The waves' (P, q).  Two sets, used in turn: a wave writes a set again only
+  // behind a barrier that every wave reaches after its last read of it, so one
+  // barrier a chunk does.
+  __shared__ f32x2 pq[2][W][64];
+  const Where w(a);
+  const int t_beg = w.seg * a.seg_steps;
+  const int t_end = a.T - t_beg < a.seg_steps ? a.T : t_beg + a.seg_steps;
+  const int lim = w.end < t_end ? w.end : t_end;
+  const bool seq = !AGG && a.y != nullptr;
 
-  float carry[V], prod[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) { carry[v] = 0.f; prod[v] = 1.f; }
-  if constexpr (!AGG) start_state<V>(a, w, carry);
+  float carry = AGG ? 0.f : start_state(a, w), prod = 1.f;
 
-  const char* xb[G];
-  uint32_t xo[G];
+  const int mine = t_beg + w.wave * L;                  // this wave's first step
+  const int64_t x_at = w.base(a.xs, mine), x_step = a.xs.t * CH;
+  const uint32_t xo = w.lane_off(a.xs, sizeof(T));
+  const char* xp[G];
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    xb[g] = w.template base<T>(a, a.x[g]);
-    xo[g] = w.template lane_off<T>(a.x[g]);
-  }
-  char* yb = seq ? w.template base<T>(a, a.y) : nullptr;
-  const uint32_t yo = seq ? w.template lane_off<T>(a.y) : 0;
-  const int64_t ys = a.y.st * (int64_t)sizeof(T);
+  for (int g = 0; g < G; ++g) xp[g] = a.x[g] + x_at;
+  char* yp = seq ? a.y + w.base(a.ys, mine) : nullptr;
+  const uint32_t yo = seq ? w.lane_off(a.ys, sizeof(T)) : 0;
 
-  vec<T, V> raw[G][L];
-  auto fetch = [&](int64_t t0) {
+  T raw[G][L];
+  auto fetch = [&](int t0) {
 #pragma unroll
-    for (int g = 0; g < GA; ++g)
-      load_steps<T, V, L>(raw[g], xb[g], a.x[g].st * (int64_t)sizeof(T), xo[g], t0, lim);
-    if constexpr (!AGG && FORM == PT_SCAN_LSTM)      // o is wanted for y, or at the row's last step
-      if (seq || (t0 < w.end && w.end <= t0 + L))
-        load_steps<T, V, L>(raw[3], xb[3], a.x[3].st * (int64_t)sizeof(T), xo[3], t0, lim);
+    for (int g = 0; g < GA; ++g) load_steps(raw[g], xp[g], a.xs.t, xo, lim - t0);
+    if constexpr (!AGG && FORM == PT_SCAN_LSTM)         // o is wanted for y, or at the row's last step
+      if (seq || (t0 < w.end && w.end - t0 <= L)) load_steps(raw[3], xp[3], a.xs.t, xo, lim - t0);
+#pragma unroll
+    for (int g = 0; g < G; ++g) xp[g] += x_step;
   };
-  fetch(t_beg + w.wave * L);
+  fetch(mine);
 
   int par = 0;
-  for (int64_t t = t_beg; t < t_end; t += CH) {
-    const int64_t t0 = t + w.wave * L;
-    if (t >= lim) {                                   // the whole chunk is behind the row's end
+  for (int t = t_beg; t < t_end; t += CH) {
+    const int t0 = t + w.wave * L, live = lim - t0;
+    if (t >= lim) {                                     // the whole chunk is behind the row's end
       if (!seq) break;
-      if (w.on) {
-#pragma unroll
-        for (int l = 0; l < L; ++l)
-          if (t0 + l < t_end) store<T, V>(yb + (t0 + l) * ys, yo, (vec<T, V>)(0));
-      }
+      if (w.on) store_steps(raw[0], yp, a.ys.t, yo, 0, t_end - t0);
+      yp += a.ys.t * CH;
       continue;
     }
-    if constexpr (!AGG)
-      if (a.saved && t > 0 && w.wave == 0 && w.on) {
-        float* s = a.saved + (t / CH - 1) * a.cols_all + w.state;
-#pragma unroll
-        for (int v = 0; v < V; ++v) s[v] = carry[v];
-      }
-    float A[L][V], B[L][V];
-    vec<T, V> o[L];
+    float A[L], B[L];
+    T o[L];
 #pragma unroll
     for (int l = 0; l < L; ++l) {
-      const bool live = t0 + l < lim;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float s, sm, d;
-        if constexpr (FORM == PT_SCAN_LEAKY) {
-          logistic<ACC>((float)raw[0][l][v], s, sm);
-          A[l][v] = live ? sm : 1.f;
-          B[l][v] = live ? s * (float)raw[1][l][v] : 0.f;
-        } else {
-          logistic<ACC>((float)raw[1][l][v], s, sm);
-          A[l][v] = live ? s : 1.f;
-          logistic<ACC>((float)raw[0][l][v], s, sm);
-          B[l][v] = live ? s * tanh_d<ACC>((float)raw[2][l][v], d) : 0.f;
-        }
-      }
+      coefs<FORM, T>((float)raw[0][l], (float)raw[1][l], GA > 2 ? (float)raw[GA - 1][l] : 0.f, A[l], B[l]);
       if constexpr (!AGG && FORM == PT_SCAN_LSTM) o[l] = raw[3][l];
     }
     if (t + CH < lim) fetch(t0 + CH);
+    if (live < L) {                                     // behind the row's end the state stays
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+        if (l >= live) { A[l] = 1.f; B[l] = 0.f; }
+    }
 
-    float cin[V];
-    if constexpr (W == 1) {
+    float cin = carry;
+    if constexpr (W > 1) {
+      f32x2 own = {A[0], B[0]};
 #pragma unroll
-      for (int v = 0; v < V; ++v) cin[v] = carry[v];
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float p = 1.f, q = 0.f;
-#pragma unroll
-        for (int l = 0; l < L; ++l) {
-          q = __builtin_fmaf(A[l][v], q, B[l][v]);
-          p *= A[l][v];
-        }
-        pq[par][w.wave][v][0][w.lane] = p;
-        pq[par][w.wave][v][1][w.lane] = q;
-      }
+      for (int l = 1; l < L; ++l) own = f32x2{own[0] * A[l], __builtin_fmaf(A[l], own[1], B[l])};
+      pq[par][w.wave][w.lane] = own;
       lds_barrier();
-      compose<W, V>(pq[par], w.wave, w.lane, carry, cin);
-      if constexpr (AGG) {
+      // compose: the state before this wave's steps, and the one after the chunk
+      const int wave = here(w.wave);
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int k = 0; k < W; ++k) prod[v] *= pq[par][k][v][0][w.lane];
+      for (int k = 0; k < W; ++k) {
+        const f32x2 e = pq[par][k][w.lane];
+        cin = k == wave ? carry : cin;
+        carry = __builtin_fmaf(e[0], carry, e[1]);
+        if constexpr (AGG) prod *= e[0];
       }
       par ^= 1;
+      if constexpr (!AGG)                               // where the backward's chunks begin
+        if (a.saved && (w.wave == 0 || w.wave == W / 2) && t0 > 0 && t0 < a.T && w.on)
+          a.saved[(t0 / (CH / 2) - 1) * a.cols_all + w.state] = cin;
     }
     if constexpr (AGG) continue;
 
-    const bool has_last = t0 < w.end && w.end <= t0 + L;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
-      vec<T, V> out;
-      float yl[V];
+    for (int l = 0; l < L; ++l) B[l] = cin = __builtin_fmaf(A[l], cin, B[l]);   // the states
+    if constexpr (W == 1) carry = cin;
+    if constexpr (FORM == PT_SCAN_LSTM) {
+      const bool has_last = t0 < w.end && w.end - t0 <= L;
+      if (seq || has_last) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        cin[v] = __builtin_fmaf(A[l][v], cin[v], B[l][v]);
-        yl[v] = cin[v];
-      }
-      if constexpr (!AGG) {
-        if constexpr (FORM == PT_SCAN_LSTM) {
-          if (seq || has_last) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              float s, sm, d;
-              logistic<ACC>((float)o[l][v], s, sm);
-              yl[v] = s * tanh_d<ACC>(cin[v], d);
-            }
-            if (t0 + l == w.end - 1 && a.h_last && w.on) {
-#pragma unroll
-              for (int v = 0; v < V; ++v) a.h_last[w.state + v] = yl[v];
-            }
-          }
+        for (int l = 0; l < L; ++l) {
+          float d;
+          B[l] = logistic<ACC>((float)o[l]).s * tanh_d<ACC>(B[l], d);
         }
-        if (seq && w.on && t0 + l < t_end) {
+        if (has_last && a.h_last && w.on) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) out[v] = (T)(t0 + l < lim ? yl[v] : 0.f);
-          store<T, V>(yb + (t0 + l) * ys, yo, out);
+          for (int l = 0; l < L; ++l)
+            if (t0 + l == w.end - 1) a.h_last[w.state] = B[l];
         }
       }
     }
-    if constexpr (W == 1) {
+    if (seq) {
+      T out[L];
 #pragma unroll
-      for (int v = 0; v < V; ++v) carry[v] = cin[v];
+      for (int l = 0; l < L; ++l) out[l] = (T)B[l];
+      if (w.on) store_steps(out, yp, a.ys.t, yo, live, t_end - t0);
+      yp += a.ys.t * CH;
     }
   }
 
   if (w.wave != 0 || !w.on) return;
   if constexpr (AGG) {
-    float* p = a.agg + 2 * (w.seg * a.cols_all + w.state);
-#pragma unroll
-    for (int v = 0; v < V; ++v) { p[2 * v] = prod[v]; p[2 * v + 1] = carry[v]; }
+    ((f32x2*)a.agg)[w.seg * a.cols_all + w.state] = f32x2{prod, carry};
   } else if (w.seg == a.segs - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (a.c_last) a.c_last[w.state + v] = carry[v];
-      if (a.h_last && FORM == PT_SCAN_LEAKY) a.h_last[w.state + v] = carry[v];
-      if (a.h_last && FORM == PT_SCAN_LSTM && w.end == 0) a.h_last[w.state + v] = 0.f;
-    }
+    if (a.c_last) a.c_last[w.state] = carry;
+    if (a.h_last && FORM == PT_SCAN_LEAKY) a.h_last[w.state] = carry;
+    if (a.h_last && FORM == PT_SCAN_LSTM && w.end == 0) a.h_last[w.state] = 0.f;
   }
 }
 
 // Backward.  AGG: reduce a segment, from zero at its far end, to (P, q) of the
 // gradient that leaves it towards the past.
-template <int FORM, typename T, int V, int W, bool AGG>
-__global__ __launch_bounds__(64 * W) void k_scan_bwd(Args a) {
-  constexpr int G = gates_of<FORM>(), L = steps_of<FORM>(), CH = W * L;
-  constexpr bool ACC = sizeof(T) == 4;
-  // Two sets, used in turn: a wave writes a set again only behind a barrier that
-  // every wave reaches after its last read of it, so one barrier an exchange does.
-  __shared__ float pq[2][W][V][2][64];   // forward (P, q)
-  __shared__ float gq[2][W][V][64];      // backward q (its P is the same)
-  int par = 0;
-  const Where<V> w(a);
-  const int seg = AGG ? w.seg + 1 : w.seg;             // nothing is behind segment 0
-  const int64_t t_beg = seg * a.seg_steps;
-  const int64_t t_end = t_beg + a.seg_steps < a.T ? t_beg + a.seg_steps : a.T;
-  const int64_t lim = w.end < t_end ? w.end : t_end;
-  const bool has_dy = a.y.p != nullptr;
+template <int FORM, typename T, int W, bool AGG>
+__global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
+  static_assert(W > 1 || !AGG, "one wave never splits the time axis over workgroups");
+  constexpr int G = gates_of<FORM>(), L = back_steps<FORM>(), CH = W * L;
+  constexpr bool LEAKY = FORM == PT_SCAN_LEAKY, ACC = sizeof(T) == 4;
+  __shared__ f32x2 pq[2][W][64];              // forward (P, q); two sets in turn, as in the forward
+  __shared__ float gq[2][W][64];              // backward q (its P is the same)
+  const Where w(a);
+  const int seg = AGG ? w.seg + 1 : w.seg;    // nothing is behind segment 0
+  const int t_beg = seg * a.seg_steps;
+  const int t_end = a.T - t_beg < a.seg_steps ? a.T : t_beg + a.seg_steps;
+  const int lim = w.end < t_end ? w.end : t_end;
+  const bool has_dy = a.y != nullptr;
+  // lstm: whether any gradient enters through y among the L steps from t0 (without
+  // a dy it does at the row's last step alone, and o, tanh(c) matter only there)
+  auto enters = [&](int t0) { return has_dy || (a.d_h_last && t0 < w.end && w.end - t0 <= L); };
 
-  float carry[V], prod[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) { carry[v] = 0.f; prod[v] = 1.f; }
+  float carry = 0.f, prod = 1.f;
   if constexpr (!AGG) {
-    const float* end = FORM == PT_SCAN_LEAKY ? a.d_h_last : a.d_c_last;
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = end ? end[w.state + v] : 0.f;
+    const float* end = LEAKY ? a.d_h_last : a.d_c_last;
+    if (end) carry = end[w.state];
+    const f32x2* p = (const f32x2*)a.agg + w.state;
     for (int s = a.segs - 1; s > seg; --s) {
-      const float* p = a.agg + 2 * ((s - 1) * a.cols_all + w.state);
-#pragma unroll
-      for (int v = 0; v < V; ++v) carry[v] = __builtin_fmaf(p[2 * v], carry[v], p[2 * v + 1]);
+      const f32x2 e = p[(s - 1) * a.cols_all];
+      carry = __builtin_fmaf(e[0], carry, e[1]);
     }
   }
 
-  const char* xb[G];
-  char* db[G];
-  uint32_t xo[G], dof[G];
+  // chunks from the last to the first
+  int t = t_beg + (t_end - 1 - t_beg) / CH * CH;
+  const int last = t + w.wave * L;                      // this wave's first step in the last chunk
+  const int64_t x_at = w.base(a.xs, last), x_step = a.xs.t * CH;
+  const uint32_t xo = w.lane_off(a.xs, sizeof(T));
+  const int64_t d_at = AGG ? 0 : w.base(a.ds, last), d_step = a.ds.t * CH;
+  const uint32_t dof = AGG ? 0 : w.lane_off(a.ds, sizeof(T));
+  const char* xp[G];
+  char* dp[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    xb[g] = w.template base<T>(a, a.x[g]);
-    xo[g] = w.template lane_off<T>(a.x[g]);
-    db[g] = AGG ? nullptr : w.template base<T>(a, a.dx[g]);
-    dof[g] = AGG ? 0 : w.template lane_off<T>(a.dx[g]);
+    xp[g] = a.x[g] + x_at;
+    dp[g] = AGG ? nullptr : a.dx[g] + d_at;
   }
-  const char* yb = has_dy ? w.template base<T>(a, a.y) : nullptr;
-  const uint32_t yo = has_dy ? w.template lane_off<T>(a.y) : 0;
+  const char* yp = has_dy ? a.y + w.base(a.ys, last) : nullptr;
+  const uint32_t yo = has_dy ? w.lane_off(a.ys, sizeof(T)) : 0;
 
-  vec<T, V> raw[G][L], rdy[L];
-  float nst[V];                                         // the state before the fetched chunk
-  auto fetch = [&](int64_t t) {
-    const int64_t t0 = t + w.wave * L;
+  T raw[G][L], rdy[L];
+  float nst = 0.f;                                      // the state before the fetched chunk
+  auto fetch = [&](int tc) {
+    const int t0 = tc + w.wave * L, live = lim - t0;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-      load_steps<T, V, L>(raw[g], xb[g], a.x[g].st * (int64_t)sizeof(T), xo[g], t0, lim);
-    if (has_dy)
-      load_steps<T, V, L>(rdy, yb, a.y.st * (int64_t)sizeof(T), yo, t0, lim);
-    const float* s = t > 0 ? a.saved + (t / CH - 1) * a.cols_all : a.h0;
+    for (int g = 0; g < (LEAKY ? AGG ? 1 : 2 : 3); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, live);
+    if constexpr (!LEAKY)
+      if (enters(t0)) load_steps(raw[3], xp[3], a.xs.t, xo, live);
+    if (has_dy) load_steps(rdy, yp, a.ys.t, yo, live);
+    if constexpr (!(AGG && LEAKY)) {
+      const float* s = tc > 0 ? a.saved + (tc / CH - 1) * a.cols_all : a.h0;
+      nst = s ? s[w.state] : 0.f;
+    }
 #pragma unroll
-    for (int v = 0; v < V; ++v) nst[v] = s ? s[w.state + v] : 0.f;
+    for (int g = 0; g < G; ++g) xp[g] -= x_step;
+    if (has_dy) yp -= a.ys.t * CH;
   };
 #pragma unroll
-  for (int l = 0; l < L; ++l) rdy[l] = 0;
+  for (int l = 0; l < L; ++l) rdy[l] = (T)0.f;
 
-  // chunks from the last to the first; those behind the row's end only clear dx
-  int64_t t = t_beg + (t_end - 1 - t_beg) / CH * CH;
-  for (; t >= t_beg && t >= lim; t -= CH) {
-    if constexpr (!AGG) {
-      if (w.on)
+  for (; t >= t_beg && t >= lim; t -= CH) {             // behind the row's end dx is only cleared
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
-          const int64_t tt = t + w.wave * L + l;
-          if (tt < t_end)
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-              store<T, V>(db[g] + tt * a.dx[g].st * (int64_t)sizeof(T), dof[g], (vec<T, V>)(0));
-        }
+    for (int g = 0; g < G; ++g) {
+      xp[g] -= x_step;
+      if constexpr (!AGG) {
+        if (w.on) store_steps(rdy, dp[g], a.ds.t, dof, 0, t_end - (t + w.wave * L));
+        dp[g] -= d_step;
+      }
     }
+    if (has_dy) yp -= a.ys.t * CH;
   }
   if (t >= t_beg) fetch(t);
+  int par = 0;
   for (; t >= t_beg; t -= CH) {
-    const int64_t t0 = t + w.wave * L;
-    float A[L][V], B[L][V], D[L][V];                    // a; b, then the state before the step; dy
-    float K0[L][V], K1[L][V], K2[L][V];                 // what the gradients are made of
-    float O[L][V], OD[L][V];                            // lstm: s(o), s(o) s(-o)
-    float st[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) st[v] = nst[v];
+    const int t0 = t + w.wave * L, live = lim - t0;
+    // a; what the gradients are made of; dy, then dL/dh_t through y_t
+    float A[L], K0[L], K1[L], D[L];
+    float B[L], K2[L];                                  // lstm
+    T o[L];
+    float cin = nst;
 #pragma unroll
     for (int l = 0; l < L; ++l) {
-      const bool live = t0 + l < lim;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float s, sm, d;
-        D[l][v] = live ? (float)rdy[l][v] : 0.f;
-        if constexpr (FORM == PT_SCAN_LEAKY) {
-          const float n = (float)raw[1][l][v];
-          logistic<ACC>((float)raw[0][l][v], s, sm);
-          A[l][v] = live ? sm : 1.f;
-          B[l][v] = live ? s * n : 0.f;
-          K0[l][v] = n;
-          K1[l][v] = s;
-        } else {
-          logistic<ACC>((float)raw[1][l][v], s, sm);
-          A[l][v] = live ? s : 1.f;
-          K1[l][v] = s * sm;                            // d f
-          logistic<ACC>((float)raw[0][l][v], s, sm);
-          const float th = tanh_d<ACC>((float)raw[2][l][v], d);
-          B[l][v] = live ? s * th : 0.f;
-          K0[l][v] = th * s * sm;                       // d i
-          K2[l][v] = s * d;                             // d n
-          logistic<ACC>((float)raw[3][l][v], s, sm);
-          O[l][v] = s;
-          OD[l][v] = s * sm;
-          if (a.d_h_last && t0 + l == w.end - 1) D[l][v] += a.d_h_last[w.state + v];
+      D[l] = (float)rdy[l];
+      if constexpr (LEAKY) {
+        const Logistic z = logistic<ACC>((float)raw[0][l]);
+        A[l] = z.sm;
+        if constexpr (!AGG) {
+          K1[l] = z.s;
+          K0[l] = (float)raw[1][l];
         }
+      } else {
+        const Logistic f = logistic<ACC>((float)raw[1][l]), i = logistic<ACC>((float)raw[0][l]);
+        float d;
+        const float th = tanh_d<ACC>((float)raw[2][l], d);
+        A[l] = f.s;
+        B[l] = i.s * th;
+        K0[l] = i.p * th;
+        K1[l] = f.p;
+        K2[l] = i.s * d;
+        o[l] = raw[3][l];
       }
     }
-    if (t - CH >= t_beg) fetch(t - CH);
+    if (t > t_beg) fetch(t - CH);
+    if (live < L) {                                     // behind the row's end: h' = h, dx = 0
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+        if (l >= live) {
+          A[l] = 1.f;
+          if constexpr (!LEAKY) B[l] = 0.f;
+          else if constexpr (!AGG) K1[l] = 0.f;
+        }
+    }
 
-    float cin[V], gin[V];
+    float gin = carry;
     if constexpr (W > 1) {
+      f32x2 own = {A[0], 0.f};
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float p = 1.f, q = 0.f, g = 0.f;
+      for (int l = 1; l < L; ++l) own[0] *= A[l];
+      if constexpr (!LEAKY || !AGG) {
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
-          q = __builtin_fmaf(A[l][v], q, B[l][v]);
-          p *= A[l][v];
-        }
-        pq[par][w.wave][v][0][w.lane] = p;
-        pq[par][w.wave][v][1][w.lane] = q;
-        if constexpr (FORM == PT_SCAN_LEAKY) {          // y = h: dy needs no state
-#pragma unroll
-          for (int l = L - 1; l >= 0; --l) g = A[l][v] * (D[l][v] + g);
-          gq[par][w.wave][v][w.lane] = g;
-        }
+        for (int l = 0; l < L; ++l) own[1] = __builtin_fmaf(A[l], own[1], LEAKY ? K1[l] * K0[l] : B[l]);
       }
-      lds_barrier();
-      compose<W, V>(pq[par], w.wave, w.lane, st, cin);
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) cin[v] = st[v];
-    }
-
-    // the states, forward; B becomes the state before each step
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      vec<T, V> dO;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float h = __builtin_fmaf(A[l][v], cin[v], B[l][v]);
-        B[l][v] = cin[v];
-        cin[v] = h;
-        if constexpr (FORM == PT_SCAN_LSTM) {
-          float d;
-          const float th = tanh_d<ACC>(h, d);
-          dO[v] = (T)(t0 + l < lim ? D[l][v] * th * OD[l][v] : 0.f);
-          D[l][v] *= O[l][v] * d;
-        }
-      }
-      if constexpr (FORM == PT_SCAN_LSTM && !AGG)
-        if (w.on && t0 + l < t_end)
-          store<T, V>(db[3] + (t0 + l) * a.dx[3].st * (int64_t)sizeof(T), dof[3], dO);
-    }
-    if constexpr (W > 1 && FORM == PT_SCAN_LSTM) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
+      pq[par][w.wave][w.lane] = own;
+      if constexpr (LEAKY) {                            // y = h: dy needs no state
         float g = 0.f;
 #pragma unroll
-        for (int l = L - 1; l >= 0; --l) g = A[l][v] * (D[l][v] + g);
-        gq[par][w.wave][v][w.lane] = g;
+        for (int l = L - 1; l >= 0; --l) g = A[l] * (D[l] + g);
+        gq[par][w.wave][w.lane] = g;
       }
       lds_barrier();
+      if constexpr (!(AGG && LEAKY)) {
+        const int wave = here(w.wave);
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) {
+          const f32x2 e = pq[par][k][w.lane];
+          cin = k < wave ? __builtin_fmaf(e[0], cin, e[1]) : cin;
+        }
+      }
+    }
+
+    // the states, forward
+    if constexpr (LEAKY) {
+      if constexpr (!AGG) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+          const float n = K0[l], s = K1[l];
+          K0[l] = (n - cin) * (s * A[l]);
+          cin = __builtin_fmaf(A[l], cin, s * n);
+        }
+      }
+    } else {
+      T out[L];
+      if (enters(t0)) {
+        if (a.d_h_last && t0 < w.end && w.end - t0 <= L) {
+          const float e = a.d_h_last[w.state];
+#pragma unroll
+          for (int l = 0; l < L; ++l) D[l] += t0 + l == w.end - 1 ? e : 0.f;
+        }
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+          K1[l] *= cin;
+          cin = __builtin_fmaf(A[l], cin, B[l]);
+          const Logistic g = logistic<ACC>((float)o[l]);
+          float d;
+          const float th = tanh_d<ACC>(cin, d);
+          out[l] = (T)(D[l] * th * g.p);
+          D[l] *= g.s * d;
+        }
+      } else {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+          K1[l] *= cin;
+          cin = __builtin_fmaf(A[l], cin, B[l]);
+          out[l] = (T)0.f;
+        }
+      }
+      if constexpr (!AGG) {
+        if (w.on) store_steps(out, dp[3], a.ds.t, dof, live, t_end - t0);
+        dp[3] -= d_step;
+      }
+      if constexpr (W > 1) {
+        float g = 0.f;
+#pragma unroll
+        for (int l = L - 1; l >= 0; --l) g = A[l] * (D[l] + g);
+        gq[par][w.wave][w.lane] = g;
+        lds_barrier();
+      }
     }
     if constexpr (W > 1) {
+      const int wave = here(w.wave);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float c = carry[v];
-#pragma unroll
-        for (int k = W - 1; k >= 0; --k) {
-          gin[v] = k == w.wave ? c : gin[v];
-          const float p = pq[par][k][v][0][w.lane];
-          if constexpr (AGG) prod[v] *= p;
-          c = __builtin_fmaf(p, c, gq[par][k][v][w.lane]);
-        }
-        carry[v] = c;
+      for (int k = W - 1; k >= 0; --k) {
+        const float p = pq[par][k][w.lane][0];
+        gin = k == wave ? carry : gin;
+        carry = __builtin_fmaf(p, carry, gq[par][k][w.lane]);
+        if constexpr (AGG) prod *= p;
       }
       par ^= 1;
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) gin[v] = carry[v];
     }
     if constexpr (AGG) continue;
 
+    T out[3][L];
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
-      vec<T, V> out[3];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float g = D[l][v] + gin[v];
-        const bool live = t0 + l < lim;
-        if constexpr (FORM == PT_SCAN_LEAKY) {
-          const float gs = g * K1[l][v];
-          out[0][v] = (T)(live ? gs * A[l][v] * (K0[l][v] - B[l][v]) : 0.f);
-          out[1][v] = (T)(live ? gs : 0.f);
-        } else {
-          out[0][v] = (T)(live ? g * K0[l][v] : 0.f);
-          out[1][v] = (T)(live ? g * B[l][v] * K1[l][v] : 0.f);
-          out[2][v] = (T)(live ? g * K2[l][v] : 0.f);
-        }
-        gin[v] = A[l][v] * g;
-      }
-      if constexpr (!AGG)
-        if (w.on && t0 + l < t_end) {
-#pragma unroll
-          for (int g = 0; g < G - (FORM == PT_SCAN_LSTM); ++g)
-            store<T, V>(db[g] + (t0 + l) * a.dx[g].st * (int64_t)sizeof(T), dof[g], out[g]);
-        }
+      const float g = D[l] + gin;
+      out[0][l] = (T)(g * K0[l]);
+      out[1][l] = (T)(g * K1[l]);
+      if constexpr (!LEAKY) out[2][l] = (T)(g * K2[l]);
+      gin = A[l] * g;
     }
-    if constexpr (W == 1) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) carry[v] = gin[v];
+    for (int g = 0; g < (LEAKY ? 2 : 3); ++g) {
+      if (w.on) store_steps(out[g], dp[g], a.ds.t, dof, live, t_end - t0);
+      dp[g] -= d_step;
     }
+    if constexpr (W == 1) carry = gin;
   }
 
   if (w.wave != 0 || !w.on) return;
-  if constexpr (AGG) {
-    float* p = a.agg + 2 * ((int64_t)w.seg * a.cols_all + w.state);
-#pragma unroll
-    for (int v = 0; v < V; ++v) { p[2 * v] = prod[v]; p[2 * v + 1] = carry[v]; }
-  } else if (seg == 0 && a.d_h0) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) a.d_h0[w.state + v] = carry[v];
-  }
+  if constexpr (AGG)
+    ((f32x2*)a.agg)[w.seg * a.cols_all + w.state] = f32x2{prod, carry};
+  else if (seg == 0 && a.d_h0)
+    a.d_h0[w.state] = carry;
 }
 
 // One step: element-wise, one lane per V columns.
 template <int FORM, typename T, int V>
-__global__ __launch_bounds__(256) void k_scan_step(Args a, View state) {
+__global__ __launch_bounds__(256) void k_scan_step(Args a, char* state, Strides ss) {
   constexpr int G = gates_of<FORM>();
   constexpr bool ACC = sizeof(T) == 4;
   const int64_t cols = a.C * a.N;
@@ -632,30 +623,26 @@ __global__ __launch_bounds__(256) void k_scan_step(Args a, View state) {
   if (i >= a.cols_all) return;
   const int64_t b = i / cols, j = i - b * cols;
   const int64_t c = a.C == 1 ? 0 : j / a.N, n = j - c * a.N;
-  auto at = [&](const View& v) { return b * v.sb + c * v.sc + n; };
+  auto at = [&](const Strides& s, int size) { return b * s.b + c * s.c + n * size; };
   vec<T, V> x[G], out;
 #pragma unroll
-  for (int g = 0; g < G; ++g) x[g] = *((const vec<T, V>*)((const T*)a.x[g].p + at(a.x[g])));
-  float* sp = (float*)state.p + at(state);
+  for (int g = 0; g < G; ++g) x[g] = *(const vec<T, V>*)(a.x[g] + at(a.xs, sizeof(T)));
+  char* sp = state + at(ss, 4);
   vec<float, V> h = *(const vec<float, V>*)sp;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float s, sm, d;
+    const Logistic g = logistic<ACC>((float)x[0][v]);
     if constexpr (FORM == PT_SCAN_LEAKY) {
-      logistic<ACC>((float)x[0][v], s, sm);
-      h[v] = __builtin_fmaf(sm, h[v], s * (float)x[1][v]);
+      h[v] = __builtin_fmaf(g.sm, h[v], g.s * (float)x[1][v]);
       out[v] = (T)h[v];
     } else {
-      float f, i_, o;
-      logistic<ACC>((float)x[1][v], f, sm);
-      logistic<ACC>((float)x[0][v], i_, sm);
-      logistic<ACC>((float)x[3][v], o, sm);
-      h[v] = __builtin_fmaf(f, h[v], i_ * tanh_d<ACC>((float)x[2][v], d));
-      out[v] = (T)(o * tanh_d<ACC>(h[v], d));
+      float d;
+      h[v] = __builtin_fmaf(logistic<ACC>((float)x[1][v]).s, h[v], g.s * tanh_d<ACC>((float)x[2][v], d));
+      out[v] = (T)(logistic<ACC>((float)x[3][v]).s * tanh_d<ACC>(h[v], d));
     }
   }
   *(vec<float, V>*)sp = h;
-  *((vec<T, V>*)((T*)a.y.p + at(a.y))) = out;
+  *(vec<T, V>*)(a.y + at(a.ys, sizeof(T))) = out;
 }
 
 // ------------------------------------------------------------------ host
@@ -669,8 +656,9 @@ int check(const pt_scan_desc* d) {
   if (d->dtype < PT_SCAN_F32 || d->dtype > PT_SCAN_F16) return fail(PT_SCAN_ERR_ARG, "scan: unknown dtype");
   if (d->batch < 1 || d->channels < 1 || d->steps < 1 || d->inner < 1)
     return fail(PT_SCAN_ERR_ARG, "scan: batch, channels, steps and inner must be >= 1");
+  if (d->steps > (int64_t)1 << 30) return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: steps must be at most 2^30");
   const int64_t big = (int64_t)1 << 40;
-  if (d->batch > big || d->channels > big || d->steps > big || d->inner > big ||
+  if (d->batch > big || d->channels > big || d->inner > big ||
       (double)d->batch * (double)d->channels * (double)d->inner * (double)d->steps > 1e15)
     return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: more elements than any device holds");
   if (d->inner >= ((int64_t)1 << 29))
@@ -681,28 +669,39 @@ int check(const pt_scan_desc* d) {
 // How a shape is cut; from the descriptor alone, so that forward, backward and
 // the size queries agree.
 struct Plan {
-  int W, L;
-  int64_t chunk, nchunks, segs, seg_steps;
+  int W;
+  int64_t chunk, nchunks;    // of the backward; the forward's are two of them
+  int segs, seg_steps;
 };
 
+// The waves that share a column tile, and the pieces that time is cut into, by
+// the column tiles there are.  The card holds 256 workgroups of 16 waves at a
+// time, or 512 of 8 (registers), or 1024 and more of 4:
+//   tiles > 512   4 waves.  More waves only make each chunk's exchange longer
+//                 (2048 tiles of 300 steps, leaky bf16: forward 48 us, 58 with 8;
+//                 700 of 4096: 262, 269).
+//   257 .. 512    8 waves (300 tiles of 4096 steps: 146 us, 162 with 4 or 16).
+//   129 .. 256    16 waves: one workgroup a compute unit (180 tiles: 81 us, 136
+//                 with 4, 108 with 8 in two pieces).
+//   up to 128     8 waves and 512 / tiles pieces of time, at the price of reading
+//                 the gates twice (64 tiles of 4096: 43 us, 118 unsplit, 46 with 16
+//                 waves in 4 pieces; 110 tiles: 67, and 71 in 16 waves and 2 pieces).
+// Up to 4 L steps fit a chunk of 4 waves, up to L steps one wave.
 Plan plan_of(const pt_scan_desc* d) {
   Plan p;
-  p.L = d->form == PT_SCAN_LEAKY ? 8 : 4;
-  const int64_t wide = 64 * (d->dtype == PT_SCAN_F32 ? 1 : 2);
-  const int64_t tiles = d->batch * ((d->channels * d->inner + wide - 1) / wide);
-  p.W = d->steps <= p.L ? 1 : tiles >= 1024 || d->steps <= 4 * p.L ? 4 : SPLIT_W;
-  p.chunk = (int64_t)p.W * p.L;
+  const int L = d->form == PT_SCAN_LEAKY ? back_steps<PT_SCAN_LEAKY>() : back_steps<PT_SCAN_LSTM>();
+  const int64_t tiles = d->batch * ((d->channels * d->inner + 63) / 64);
+  if (d->steps <= L) p.W = 1;
+  else if (d->steps <= 4 * L || tiles > 512) p.W = 4;
+  else p.W = tiles > 128 && tiles <= 256 ? 16 : SPLIT_W;
+  p.chunk = (int64_t)p.W * L;
   p.nchunks = (d->steps + p.chunk - 1) / p.chunk;
-  p.segs = 1;
-  if (p.W == SPLIT_W && tiles < 512) {
-    p.segs = (512 + tiles - 1) / tiles;
-    if (p.segs > p.nchunks / 2) p.segs = p.nchunks / 2;
-    if (p.segs > MAX_SEGS) p.segs = MAX_SEGS;
-    if (p.segs < 1) p.segs = 1;
-  }
-  const int64_t per = (p.nchunks + p.segs - 1) / p.segs;
-  p.segs = (p.nchunks + per - 1) / per;
-  p.seg_steps = per * p.chunk;
+  const int64_t pairs = (p.nchunks + 1) / 2;
+  int64_t segs = 1;
+  if (p.W == SPLIT_W && tiles <= 128) segs = std::min<int64_t>(std::min<int64_t>(512 / tiles, pairs), MAX_SEGS);
+  const int64_t per = (pairs + segs - 1) / segs;
+  p.segs = (int)((pairs + per - 1) / per);
+  p.seg_steps = (int)std::min<int64_t>(per * 2 * p.chunk, (int64_t)1 << 30);
   return p;
 }
 
@@ -710,7 +709,7 @@ Plan plan_of(const pt_scan_desc* d) {
 pt_scan_view tidy(const pt_scan_desc* d, const pt_scan_view& v) {
   return pt_scan_view{v.data, d->batch == 1 ? 0 : v.sb, d->channels == 1 ? 0 : v.sc, d->steps == 1 ? 0 : v.st};
 }
-View view_of(const pt_scan_view& v) { return View{(char*)v.data, v.sb, v.sc, v.st}; }
+Strides bytes_of(const pt_scan_view& v, int size) { return Strides{v.sb * size, v.sc * size, v.st * size}; }
 
 // Both halves of the alignment rule: V elements of a lane are one load only if
 // every stride and the base keep them aligned and V divides the inner axis.
@@ -723,75 +722,96 @@ bool spans32(const pt_scan_desc* d, const pt_scan_view& v, int size) {
   return v.sc >= 0 && s < 2147483648.0;
 }
 
-template <int FORM, typename T, int V, int W>
+template <int FORM, typename T, int W>
 int launch_fwd(Args a, int64_t blocks, hipStream_t s) {
   if constexpr (W == SPLIT_W)
     if (a.segs > 1) {
       const int64_t n = blocks / a.segs * (a.segs - 1);
-      hipLaunchKernelGGL((k_scan_fwd<FORM, T, V, W, true>), dim3((unsigned)n), dim3(64 * W), 0, s, a);
+      hipLaunchKernelGGL((k_scan_fwd<FORM, T, W, true>), dim3((unsigned)n), dim3(64 * W), 0, s, a);
     }
-  hipLaunchKernelGGL((k_scan_fwd<FORM, T, V, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
+  hipLaunchKernelGGL((k_scan_fwd<FORM, T, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
   return hipGetLastError() == hipSuccess ? 0 : fail(PT_SCAN_ERR_HIP, "scan: forward launch failed");
 }
 
-template <int FORM, typename T, int V, int W>
+template <int FORM, typename T, int W>
 int launch_bwd(Args a, int64_t blocks, hipStream_t s) {
   if constexpr (W == SPLIT_W)
     if (a.segs > 1) {
       const int64_t n = blocks / a.segs * (a.segs - 1);
-      hipLaunchKernelGGL((k_scan_bwd<FORM, T, V, W, true>), dim3((unsigned)n), dim3(64 * W), 0, s, a);
+      hipLaunchKernelGGL((k_scan_bwd<FORM, T, W, true>), dim3((unsigned)n), dim3(64 * W), 0, s, a);
     }
-  hipLaunchKernelGGL((k_scan_bwd<FORM, T, V, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
+  hipLaunchKernelGGL((k_scan_bwd<FORM, T, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
   return hipGetLastError() == hipSuccess ? 0 : fail(PT_SCAN_ERR_HIP, "scan: backward launch failed");
 }
 
-template <int FORM, typename T, int V>
+template <int FORM, typename T>
 int launch_w(const Plan& p, const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
   switch (p.W) {
-    case 1: return bwd ? launch_bwd<FORM, T, V, 1>(a, blocks, s) : launch_fwd<FORM, T, V, 1>(a, blocks, s);
-    case 4: return bwd ? launch_bwd<FORM, T, V, 4>(a, blocks, s) : launch_fwd<FORM, T, V, 4>(a, blocks, s);
-    default: return bwd ? launch_bwd<FORM, T, V, SPLIT_W>(a, blocks, s) : launch_fwd<FORM, T, V, SPLIT_W>(a, blocks, s);
+    case 1: return bwd ? launch_bwd<FORM, T, 1>(a, blocks, s) : launch_fwd<FORM, T, 1>(a, blocks, s);
+    case 16: return bwd ? launch_bwd<FORM, T, 16>(a, blocks, s) : launch_fwd<FORM, T, 16>(a, blocks, s);
+    case 4: return bwd ? launch_bwd<FORM, T, 4>(a, blocks, s) : launch_fwd<FORM, T, 4>(a, blocks, s);
+    default: return bwd ? launch_bwd<FORM, T, SPLIT_W>(a, blocks, s) : launch_fwd<FORM, T, SPLIT_W>(a, blocks, s);
   }
 }
 
 template <int FORM>
-int launch_t(int dtype, int V, const Plan& p, const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
-  if (dtype == PT_SCAN_F32) return launch_w<FORM, float, 1>(p, a, blocks, bwd, s);
-  if (dtype == PT_SCAN_BF16)
-    return V == 2 ? launch_w<FORM, __bf16, 2>(p, a, blocks, bwd, s) : launch_w<FORM, __bf16, 1>(p, a, blocks, bwd, s);
-  return V == 2 ? launch_w<FORM, _Float16, 2>(p, a, blocks, bwd, s) : launch_w<FORM, _Float16, 1>(p, a, blocks, bwd, s);
+int launch_t(int dtype, const Plan& p, const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
+  if (dtype == PT_SCAN_F32) return launch_w<FORM, float>(p, a, blocks, bwd, s);
+  if (dtype == PT_SCAN_BF16) return launch_w<FORM, __bf16>(p, a, blocks, bwd, s);
+  return launch_w<FORM, _Float16>(p, a, blocks, bwd, s);
 }
 
-int run(const pt_scan_desc* d, const Plan& p, Args& a, const pt_scan_view* views, int nviews, bool bwd,
-        hipStream_t s) {
-  const int size = elem_size(d->dtype);
-  int V = size == 4 || d->inner % 2 ? 1 : 2;
-  bool grouped = true;
-  for (int i = 0; i < nviews; ++i) {
-    if (V > 1 && !aligned(views[i], V, size)) V = 1;
-    if ((uintptr_t)views[i].data % size) return fail(PT_SCAN_ERR_ARG, "scan: a tensor is not aligned to its elements");
-    if (!spans32(d, views[i], size)) grouped = false;
+// The tensors of a call, checked.
+struct Tensors {
+  const pt_scan_desc* d;
+  int size;
+  bool wide;                 // 16 bytes of neighbours lie together and aligned in every one
+  bool grouped = true;       // 32-bit offsets reach over the channels of a step
+  int rc = 0;
+
+  explicit Tensors(const pt_scan_desc* desc) : d(desc), size(elem_size(desc->dtype)) {
+    wide = d->inner % (16 / size) == 0;
   }
+  // `count` views of one kind: their pointers and shared strides
+  template <typename P> void take(const pt_scan_view* v, int count, P** ptr, Strides& s, int elem) {
+    if (rc) return;
+    for (int g = 0; g < count; ++g) {
+      const pt_scan_view t = tidy(d, v[g]), first = tidy(d, v[0]);
+      if (!t.data) { rc = fail(PT_SCAN_ERR_ARG, "scan: null pointer"); return; }
+      if ((uintptr_t)t.data % elem) { rc = fail(PT_SCAN_ERR_ARG, "scan: a tensor is not aligned to its elements"); return; }
+      if (t.sb != first.sb || t.sc != first.sc || t.st != first.st) {
+        rc = fail(PT_SCAN_ERR_UNSUPPORTED, "scan: the gates must share their strides");
+        return;
+      }
+      wide = wide && aligned(t, 16 / size, elem);
+      grouped = grouped && spans32(d, t, elem);
+      ptr[g] = (P*)t.data;
+      s = bytes_of(t, elem);
+    }
+  }
+};
+
+int run(const pt_scan_desc* d, const Plan& p, const Tensors& ts, Args& a, bool bwd, hipStream_t s) {
   // Columns of one channel at a time where the inner axis fills whole tiles, or
   // where the channels of a step reach over more than a 32-bit offset.
-  if (d->inner % (64 * V) == 0) grouped = false;
-  if ((double)d->channels * (double)d->inner >= 2147483648.0) grouped = false;
+  const bool grouped = ts.grouped && d->inner % 64 != 0 &&
+                       (double)d->channels * (double)d->inner < 2147483648.0;
   a.C = d->channels;
   a.N = d->inner;
-  a.T = d->steps;
+  a.T = (int)d->steps;
   a.cols_all = d->batch * d->channels * d->inner;
   a.cg = grouped ? d->channels : 1;
   a.groups = d->channels / a.cg;
   a.outer = d->batch * a.groups;
-  a.segs = (int)p.segs;
+  a.segs = p.segs;
   a.seg_steps = p.seg_steps;
-  const int64_t tiles = (a.cg * a.N + 64 * V - 1) / (64 * V);
+  const int64_t tiles = (a.cg * a.N + 63) / 64;
   a.tiles = (int)tiles;
   if ((double)tiles * (double)a.outer * (double)p.segs > 2147483647.0)
     return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: too many columns for one launch");
   const int64_t blocks = tiles * a.outer * p.segs;
-  return d->form == PT_SCAN_LEAKY ? launch_t<PT_SCAN_LEAKY>(d->dtype, V, p, a, blocks, bwd, s)
-                                  : launch_t<PT_SCAN_LSTM>(d->dtype, V, p, a, blocks, bwd, s);
+  return d->form == PT_SCAN_LEAKY ? launch_t<PT_SCAN_LEAKY>(d->dtype, p, a, blocks, bwd, s)
+                                  : launch_t<PT_SCAN_LSTM>(d->dtype, p, a, blocks, bwd, s);
 }
 
 }  // namespace
@@ -820,20 +840,15 @@ int pt_scan_forward(const pt_scan_desc* d, const pt_scan_view* x, const float* h
   if (!x) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
   const Plan p = plan_of(d);
   Args a{};
-  pt_scan_view views[5];
-  int n = 0;
-  for (int g = 0; g < gates(d->form); ++g) {
-    if (!x[g].data) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
-    a.x[g] = view_of(views[n++] = tidy(d, x[g]));
-  }
-  if (y && y->data) {
-    a.y = view_of(views[n++] = tidy(d, *y));
-  }
+  Tensors ts(d);
+  ts.take(x, gates(d->form), a.x, a.xs, ts.size);
+  if (y && y->data) ts.take(y, 1, &a.y, a.ys, ts.size);
+  if (ts.rc) return ts.rc;
   if (p.segs > 1 && !workspace) return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace");
   a.h0 = h0; a.len = lengths; a.h_last = h_last; a.c_last = c_last;
   a.saved = p.nchunks > 1 ? (float*)saved : nullptr;
   a.agg = (float*)workspace;
-  return run(d, p, a, views, n, false, (hipStream_t)stream);
+  return run(d, p, ts, a, false, (hipStream_t)stream);
 }
 
 int pt_scan_backward(const pt_scan_desc* d, const pt_scan_view* x, const float* h0, const int64_t* lengths,
@@ -843,52 +858,41 @@ int pt_scan_backward(const pt_scan_desc* d, const pt_scan_view* x, const float* 
   if (!x || !dx) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
   const Plan p = plan_of(d);
   Args a{};
-  pt_scan_view views[9];
-  int n = 0;
-  for (int g = 0; g < gates(d->form); ++g) {
-    if (!x[g].data || !dx[g].data) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
-    a.x[g] = view_of(views[n++] = tidy(d, x[g]));
-    a.dx[g] = view_of(views[n++] = tidy(d, dx[g]));
-  }
-  if (dy && dy->data) {
-    a.y = view_of(views[n++] = tidy(d, *dy));
-  }
+  Tensors ts(d);
+  ts.take(x, gates(d->form), a.x, a.xs, ts.size);
+  ts.take(dx, gates(d->form), a.dx, a.ds, ts.size);
+  if (dy && dy->data) ts.take(dy, 1, &a.y, a.ys, ts.size);
+  if (ts.rc) return ts.rc;
   if (p.nchunks > 1 && !saved) return fail(PT_SCAN_ERR_ARG, "scan: the backward needs the forward's saved states");
   if (p.segs > 1 && !workspace) return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace");
   a.h0 = h0; a.len = lengths; a.d_h_last = d_h_last; a.d_c_last = d_c_last; a.d_h0 = d_h0;
   a.saved = (float*)saved;
   a.agg = (float*)workspace;
-  return run(d, p, a, views, n, true, (hipStream_t)stream);
+  return run(d, p, ts, a, true, (hipStream_t)stream);
 }
 
 int pt_scan_step(const pt_scan_desc* d, const pt_scan_view* x, const pt_scan_view* state, const pt_scan_view* y,
                  pt_scan_stream_t stream) {
   if (int rc = check(d)) return rc;
-  if (!x || !state || !y || !state->data || !y->data) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
+  if (!x || !state || !y) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
   if (d->steps != 1) return fail(PT_SCAN_ERR_ARG, "scan: a step has steps = 1");
-  const int size = elem_size(d->dtype), wide = 16 / size;
   Args a{};
-  const pt_scan_view yv = tidy(d, *y), sv = tidy(d, *state);
-  bool al = d->inner % wide == 0 && aligned(yv, wide, size) && aligned(sv, wide, 4);
-  for (int g = 0; g < gates(d->form); ++g) {
-    if (!x[g].data) return fail(PT_SCAN_ERR_ARG, "scan: null pointer");
-    const pt_scan_view xv = tidy(d, x[g]);
-    a.x[g] = view_of(xv);
-    al = al && aligned(xv, wide, size);
-    if ((uintptr_t)x[g].data % size) return fail(PT_SCAN_ERR_ARG, "scan: a tensor is not aligned to its elements");
-  }
-  if ((uintptr_t)y->data % size || (uintptr_t)state->data % 4)
-    return fail(PT_SCAN_ERR_ARG, "scan: a tensor is not aligned to its elements");
-  a.y = view_of(yv);
+  Tensors ts(d);
+  char* sp = nullptr;
+  Strides ss{};
+  ts.take(x, gates(d->form), a.x, a.xs, ts.size);
+  ts.take(y, 1, &a.y, a.ys, ts.size);
+  ts.take(state, 1, &sp, ss, 4);
+  if (ts.rc) return ts.rc;
+  const bool al = ts.wide;
   a.C = d->channels;
   a.N = d->inner;
   a.cols_all = d->batch * d->channels * d->inner;
-  const int V = al ? wide : 1;
+  const int V = al ? 16 / ts.size : 1;
   const int64_t blocks = (a.cols_all / V + 255) / 256;
   if (blocks > 2147483647) return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: too many columns for one launch");
-  const View st = view_of(sv);
   hipStream_t s = (hipStream_t)stream;
-#define PT_STEP(F, T, V_) hipLaunchKernelGGL((k_scan_step<F, T, V_>), dim3((unsigned)blocks), dim3(256), 0, s, a, st)
+#define PT_STEP(F, T, V_) hipLaunchKernelGGL((k_scan_step<F, T, V_>), dim3((unsigned)blocks), dim3(256), 0, s, a, sp, ss)
 #define PT_STEP_T(F)                                                                     \
   do {                                                                                   \
     if (d->dtype == PT_SCAN_F32) { if (al) PT_STEP(F, float, 4); else PT_STEP(F, float, 1); }        \

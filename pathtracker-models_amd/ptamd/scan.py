@@ -180,6 +180,12 @@ def _chunks(x, gates, gate_dim):
     return [x.narrow(gate_dim, g * w, w) for g in range(gates)]
 
 
+def _alike(gates):
+    """The gates with one set of strides, as the library reads them."""
+    st = gates[0].stride()
+    return gates if all(g.stride() == st for g in gates) else [g.contiguous() for g in gates]
+
+
 # ---------------------------------------------------------------- whole sequences
 
 def _fold(tensors, dim, ragged):
@@ -190,7 +196,7 @@ def _fold(tensors, dim, ragged):
 def _forward(form, dim, gate_dim, want_seq, lengths, h0, xs, keep):
     """(y, h_last, c_last, saved): the library's forward; ``keep`` for a backward."""
     lib = load()
-    gates = _chunks(xs[0], GATES[form], gate_dim) if gate_dim is not None else list(xs)
+    gates = _alike(_chunks(xs[0], GATES[form], gate_dim) if gate_dim is not None else list(xs))
     x0 = gates[0]
     shape, device = x0.shape, x0.device
     seq = [torch.empty(shape, dtype=x0.dtype, device=device)] if want_seq else []
@@ -237,8 +243,8 @@ class GatedScanFn(torch.autograd.Function):
             whole = torch.empty_like(xs[0])
             dgates = _chunks(whole, GATES[form], gate_dim)
         else:
-            gates = xs
-            whole, dgates = None, [torch.empty_like(x) for x in xs]
+            gates = _alike(xs)
+            whole, dgates = None, [torch.empty_like(g) for g in gates]
         if dy is not None and any(st == 0 and n > 1 for st, n in zip(dy.stride(), dy.shape)):
             dy = dy.contiguous()             # an expanded dy (of a sum, a mean) has no dense axis
         extra = [dy] if dy is not None else []
@@ -388,7 +394,7 @@ def gated_scan_step(x, state, *, form="leaky", gate_dim=1):
     y = torch.empty(shape, dtype=xs[0].dtype, device=state.device)
     if y.numel() == 0:
         return y
-    gates = _chunks(xs[0], GATES[form], gate_dim) if gate_dim is not None else list(xs)
+    gates = _alike(_chunks(xs[0], GATES[form], gate_dim) if gate_dim is not None else list(xs))
     if not _disjoint(shape, state.stride()):
         raise ValueError("state's elements share memory: it cannot be updated in place")
     fold = _layout(shape, None, tuple(t.stride() for t in (*gates, state, y)), False)

@@ -39,7 +39,7 @@ def test_sizes_of_the_buffers():
 @pytest.mark.parametrize("field,value,word", [
     ("form", 2, b"form"), ("form", -1, b"form"), ("dtype", 3, b"dtype"), ("dtype", -1, b"dtype"),
     ("batch", 0, b">= 1"), ("channels", 0, b">= 1"), ("steps", 0, b">= 1"), ("inner", 0, b">= 1"),
-    ("inner", 1 << 29, b"2^29"), ("steps", 1 << 60, b"more elements")])
+    ("inner", 1 << 29, b"2^29"), ("steps", (1 << 30) + 1, b"2^30"), ("batch", 1 << 60, b"more elements")])
 def test_bad_descriptors_are_refused(field, value, word):
     lib = scan.load()
     d = scan.Desc(0, 0, 2, 3, 5, 7)
@@ -64,6 +64,8 @@ def test_bad_pointers_are_refused():
     def fwd(x, work=8192):
         return lib.pt_scan_forward(r, x, None, None, None, None, None, None, work, None)
 
+    apart = (scan.View * 4)(scan.View(4096, 0, 0, 64), scan.View(4096, 0, 0, 128))
+    assert fwd(apart) == 2 and b"strides" in lib.pt_scan_last_error()
     for x, work, word in ((None, 8192, b"null"), (null, 8192, b"null"), (good, None, b"workspace"),
                           (odd, 8192, b"aligned")):
         assert fwd(x, work) == 1 and word in lib.pt_scan_last_error()
