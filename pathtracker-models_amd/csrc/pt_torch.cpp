@@ -1,0 +1,659 @@
+// pt_torch.cpp — the tensors' side of pt_scan.h and pt_clip.h (ptamd/_native.so).
+//
+// Argument checks, layouts, buffers and the autograd node of ptamd.scan and
+// ptamd.clip.  These calls are made once a token or once a step and run for a
+// few microseconds on the device; in Python the checks and the node alone took
+// 15 us (a step), 65 us (30 gradients) and 140 us (a forward and backward), so
+// they are here.  The kernels stay behind the C ABI: both libraries are opened
+// by path and called through their headers' functions.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <dlfcn.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <algorithm>
+#include <cmath>
+#include <optional>
+#include <string>
+#include <vector>
+
+#include "pt_clip.h"
+#include "pt_scan.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+// ------------------------------------------------------------------ the libraries
+
+struct Libs {
+  decltype(&pt_scan_saved_bytes) scan_saved;
+  decltype(&pt_scan_workspace_bytes) scan_work;
+  decltype(&pt_scan_forward) scan_forward;
+  decltype(&pt_scan_backward) scan_backward;
+  decltype(&pt_scan_step) scan_step;
+  decltype(&pt_scan_last_error) scan_error;
+  decltype(&pt_clip_workspace_bytes) clip_work;
+  decltype(&pt_clip_norm) clip_norm;
+  decltype(&pt_clip_grads) clip_grads;
+  decltype(&pt_clip_last_error) clip_error;
+};
+Libs lib;
+PyObject* scan_error_type = nullptr;
+PyObject* clip_error_type = nullptr;
+
+template <typename F> void find(void* so, const char* name, F& f) {
+  f = reinterpret_cast<F>(dlsym(so, name));
+  TORCH_CHECK(f, "the library lacks ", name);
+}
+
+void* open_lib(const std::string& path) {
+  void* so = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
+  TORCH_CHECK(so, path, " cannot be opened: ", dlerror());
+  return so;
+}
+
+void open_scan(const std::string& path, py::object error) {
+  void* so = open_lib(path);
+  find(so, "pt_scan_saved_bytes", lib.scan_saved);
+  find(so, "pt_scan_workspace_bytes", lib.scan_work);
+  find(so, "pt_scan_forward", lib.scan_forward);
+  find(so, "pt_scan_backward", lib.scan_backward);
+  find(so, "pt_scan_step", lib.scan_step);
+  find(so, "pt_scan_last_error", lib.scan_error);
+  scan_error_type = error.release().ptr();
+}
+
+void open_clip(const std::string& path, py::object error) {
+  void* so = open_lib(path);
+  find(so, "pt_clip_workspace_bytes", lib.clip_work);
+  find(so, "pt_clip_norm", lib.clip_norm);
+  find(so, "pt_clip_grads", lib.clip_grads);
+  find(so, "pt_clip_last_error", lib.clip_error);
+  clip_error_type = error.release().ptr();
+}
+
+// The module's own exception where Python is calling; the autograd engine's
+// threads hold no interpreter lock and pass a RuntimeError on.
+[[noreturn]] void raise(PyObject* type, const std::string& msg) {
+  if (type && PyGILState_Check()) {
+    PyErr_SetString(type, msg.c_str());
+    throw py::error_already_set();
+  }
+  throw std::runtime_error(msg);
+}
+
+void check_scan(int rc) {
+  if (rc) raise(scan_error_type, "pt_scan error " + std::to_string(rc) + ": " + lib.scan_error());
+}
+void check_clip(int rc) {
+  if (rc) raise(clip_error_type, "pt_clip error " + std::to_string(rc) + ": " + lib.clip_error());
+}
+
+template <typename S> S stream_of(const Tensor& t) {
+  return (S)c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+int type_code(at::ScalarType t) {
+  return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
+}
+
+// ------------------------------------------------------------------ layouts
+
+struct Fold {
+  int64_t b, c, n;
+  std::vector<pt_scan_view> views;       // strides; no pointers yet
+};
+
+// Dimensions lo..hi-1 as one axis of every tensor: its size and strides.
+// Axes of one element drop out.
+bool merge(const std::vector<int64_t>& size, const std::vector<std::vector<int64_t>>& st, size_t lo, size_t hi,
+           int64_t& n, std::vector<int64_t>& out) {
+  n = 1;
+  out.assign(st.size(), 0);
+  bool first = true;
+  for (size_t k = hi; k-- > lo;) {
+    if (size[k] == 1) continue;
+    for (size_t i = 0; i < st.size(); ++i) {
+      if (first) out[i] = st[i][k];
+      else if (st[i][k] != out[i] * n) return false;
+    }
+    first = false;
+    n *= size[k];
+  }
+  return true;
+}
+
+// How tensors of one shape (their strides differing) fold into [batch][channels]
+// [steps][inner], time at `dim` (-1: no time axis).  batch_first: the batch is
+// dimension 0 alone, as row ends need it.
+std::optional<Fold> fold(at::IntArrayRef sizes, int64_t dim, const std::vector<at::IntArrayRef>& strides,
+                         bool batch_first) {
+  std::vector<int64_t> size;
+  std::vector<std::vector<int64_t>> st(strides.size());
+  Fold f;
+  f.views.resize(strides.size());
+  for (size_t k = 0; k < sizes.size(); ++k) {
+    if ((int64_t)k == dim) continue;
+    size.push_back(sizes[k]);
+    for (size_t i = 0; i < strides.size(); ++i) st[i].push_back(strides[i][k]);
+  }
+  for (size_t i = 0; i < strides.size(); ++i) f.views[i].st = dim < 0 ? 0 : strides[i][dim];
+  const size_t first = batch_first ? 1 : 0;
+  size_t inner = size.size();
+  f.n = 1;
+  while (inner > first) {                // every trailing axis that all tensors hold densely
+    bool dense = true;
+    for (const auto& s : st) dense = dense && (size[inner - 1] == 1 || s[inner - 1] == f.n);
+    if (!dense) break;
+    f.n *= size[--inner];
+  }
+  std::vector<int64_t> bs, cs;
+  for (size_t cut = first; cut <= inner; ++cut)          // dimensions cut..inner-1: channels
+    if (merge(size, st, 0, cut, f.b, bs) && merge(size, st, cut, inner, f.c, cs)) {
+      for (size_t i = 0; i < st.size(); ++i) {
+        f.views[i].sb = bs[i];
+        f.views[i].sc = cs[i];
+      }
+      return f;
+    }
+  return std::nullopt;
+}
+
+// Whether no two elements share memory, for strides that nest.
+bool disjoint(at::IntArrayRef sizes, at::IntArrayRef strides) {
+  std::vector<std::pair<int64_t, int64_t>> v;
+  for (size_t k = 0; k < sizes.size(); ++k)
+    if (sizes[k] > 1) v.emplace_back(strides[k], sizes[k]);
+  std::sort(v.begin(), v.end());
+  int64_t reach = 1;
+  for (const auto& [st, n] : v) {
+    if (st < reach) return false;
+    reach += st * (n - 1);
+  }
+  return true;
+}
+
+bool expanded(const Tensor& t) {
+  for (int64_t k = 0; k < t.dim(); ++k)
+    if (t.stride(k) == 0 && t.size(k) > 1) return true;
+  return false;
+}
+
+// ------------------------------------------------------------------ the scan
+
+using Gates = std::vector<Tensor>;
+
+struct Form {
+  int code;
+  int gates;
+  bool lstm() const { return code == PT_SCAN_LSTM; }
+};
+
+Form form_of(const std::string& name) {
+  if (name == "leaky") return {PT_SCAN_LEAKY, 2};
+  TORCH_CHECK_VALUE(name == "lstm", "unknown form '", name, "': one of leaky, lstm");
+  return {PT_SCAN_LSTM, 4};
+}
+
+Gates chunks(const Tensor& x, int gates, int64_t gate_dim) {
+  const int64_t w = x.size(gate_dim) / gates;
+  Gates out;
+  for (int g = 0; g < gates; ++g) out.push_back(x.narrow(gate_dim, g * w, w));
+  return out;
+}
+
+// The gates with one set of strides, as the library reads them.
+void alike(Gates& gates) {
+  for (const auto& g : gates)
+    if (g.strides() != gates[0].strides()) {
+      for (auto& h : gates) h = h.contiguous();
+      return;
+    }
+}
+
+// The common layout of tensors, and views with their pointers.
+std::optional<Fold> fold_of(const std::vector<const Tensor*>& ts, int64_t dim, bool batch_first) {
+  std::vector<at::IntArrayRef> st;
+  for (const Tensor* t : ts) st.push_back(t->strides());
+  auto f = fold(ts[0]->sizes(), dim, st, batch_first);
+  if (f)
+    for (size_t i = 0; i < ts.size(); ++i) f->views[i].data = ts[i]->data_ptr();
+  return f;
+}
+
+void append(std::vector<const Tensor*>& v, const Gates& g) {
+  for (const auto& t : g) v.push_back(&t);
+}
+
+std::vector<int64_t> without(at::IntArrayRef sizes, int64_t dim) {
+  std::vector<int64_t> out(sizes.begin(), sizes.end());
+  out.erase(out.begin() + dim);
+  return out;
+}
+
+template <typename T> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
+
+Tensor bytes(size_t n, const Tensor& like) {
+  return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+struct Scanned {
+  Tensor y, h_last, c_last, saved;
+};
+
+Scanned forward(Form form, int64_t dim, int64_t gate_dim, bool want_seq, const Tensor& lengths, const Tensor& h0,
+                const Gates& xs, bool keep) {
+  Gates gates = gate_dim >= 0 ? chunks(xs[0], form.gates, gate_dim) : xs;
+  alike(gates);
+  const c10::DeviceGuard guard(gates[0].device());
+  const auto opts = gates[0].options();
+  const auto end = without(gates[0].sizes(), dim);
+  Scanned r;
+  if (want_seq) r.y = at::empty(gates[0].sizes(), opts);
+  auto folded = [&] {
+    std::vector<const Tensor*> ts;
+    append(ts, gates);
+    if (want_seq) ts.push_back(&r.y);
+    return fold_of(ts, dim, lengths.defined() || dim != 0);
+  };
+  auto f = folded();
+  if (!f) {                              // no common layout: dense copies have one
+    for (auto& g : gates) g = g.contiguous();
+    f = folded();
+  }
+  const pt_scan_desc d{form.code, type_code(gates[0].scalar_type()), f->b, f->c, gates[0].size(dim), f->n};
+  r.h_last = at::empty(end, opts.dtype(at::kFloat));
+  if (form.lstm()) r.c_last = at::empty(end, opts.dtype(at::kFloat));
+  if (keep) r.saved = bytes(lib.scan_saved(&d), gates[0]);
+  const Tensor work = bytes(lib.scan_work(&d), gates[0]);
+  check_scan(lib.scan_forward(&d, f->views.data(), ptr<float>(h0), ptr<int64_t>(lengths),
+                              want_seq ? &f->views[form.gates] : nullptr, ptr<float>(r.h_last), ptr<float>(r.c_last),
+                              ptr<void>(r.saved), ptr<void>(work), stream_of<pt_scan_stream_t>(gates[0])));
+  return r;
+}
+
+// y, h_last, c_last = scan(gates; h0); x: one tensor with the gates stacked along
+// gate_dim, or up to four tensors (gate_dim -1).
+struct ScanFn : torch::autograd::Function<ScanFn> {
+  using Opt = std::optional<Tensor>;
+  static constexpr int kArgs = 11;
+
+  static variable_list forward(AutogradContext* ctx, int64_t code, int64_t count, int64_t dim, int64_t gate_dim,
+                               bool want_seq, const Opt& lengths, const Opt& h0, const Opt& x0, const Opt& x1,
+                               const Opt& x2, const Opt& x3) {
+    const Form form{(int)code, (int)count};
+    Gates xs;
+    for (const Opt* x : {&x0, &x1, &x2, &x3})
+      if (x->has_value()) xs.push_back(**x);
+    const Tensor len = lengths.value_or(Tensor()), h = h0.value_or(Tensor());
+    Scanned r = ::forward(form, dim, gate_dim, want_seq, len, h, xs, true);
+    variable_list keep{len, h, r.saved};
+    keep.insert(keep.end(), xs.begin(), xs.end());
+    ctx->save_for_backward(keep);
+    ctx->saved_data["args"] = std::vector<int64_t>{code, count, dim, gate_dim, want_seq};
+    ctx->set_materialize_grads(false);
+    variable_list out;
+    if (want_seq) out.push_back(r.y);
+    out.push_back(r.h_last);
+    if (form.lstm()) out.push_back(r.c_last);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const Form form{(int)args[0], (int)args[1]};
+    const int64_t dim = args[2], gate_dim = args[3];
+    const bool want_seq = args[4] != 0;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &lengths = saved[0], &h0 = saved[1], &states = saved[2];
+    const Gates xs(saved.begin() + 3, saved.end());
+    const c10::DeviceGuard guard(xs[0].device());
+    variable_list out;
+    {
+      at::NoGradGuard no_grad;
+      out = run(form, dim, gate_dim, want_seq, lengths, h0, states, xs, grads);
+    }
+    if (at::GradMode::is_enabled()) {    // the gradients have no derivative of their own
+      auto err = std::make_shared<torch::autograd::DelayedError>(
+          "gated_scan is differentiable once: its gradients have no derivative", (int)out.size());
+      return (*err)(std::move(out));
+    }
+    return out;
+  }
+
+  static variable_list run(Form form, int64_t dim, int64_t gate_dim, bool want_seq, const Tensor& lengths,
+                           const Tensor& h0, const Tensor& states, const Gates& xs, const variable_list& grads) {
+    Tensor dy = want_seq ? grads[0] : Tensor(), dh = grads[want_seq ? 1 : 0];
+    Tensor dc = form.lstm() ? grads[want_seq ? 2 : 1] : Tensor();
+    if (dy.defined() && expanded(dy)) dy = dy.contiguous();      // (of a sum, a mean) no dense axis
+    if (dh.defined()) dh = dh.contiguous();
+    if (dc.defined()) dc = dc.contiguous();
+    Tensor whole;
+    Gates gates, dgates;
+    if (gate_dim >= 0) {
+      gates = chunks(xs[0], form.gates, gate_dim);
+      whole = at::empty_like(xs[0]);
+      dgates = chunks(whole, form.gates, gate_dim);
+    } else {
+      gates = xs;
+      alike(gates);
+      for (const auto& g : gates) dgates.push_back(at::empty_like(g));
+    }
+    auto folded = [&] {
+      std::vector<const Tensor*> ts;
+      append(ts, gates);
+      append(ts, dgates);
+      if (dy.defined()) ts.push_back(&dy);
+      return fold_of(ts, dim, lengths.defined() || dim != 0);
+    };
+    auto f = folded();
+    if (!f) {
+      whole = Tensor();
+      for (int g = 0; g < form.gates; ++g) {
+        gates[g] = gates[g].contiguous();
+        dgates[g] = at::empty_like(gates[g]);
+      }
+      if (dy.defined()) dy = dy.contiguous();
+      f = folded();
+    }
+    const pt_scan_desc d{form.code, type_code(gates[0].scalar_type()), f->b, f->c, gates[0].size(dim), f->n};
+    const Tensor dh0 = h0.defined() && h0.requires_grad() ? at::empty_like(h0) : Tensor();
+    const Tensor work = bytes(lib.scan_work(&d), gates[0]);
+    check_scan(lib.scan_backward(&d, f->views.data(), ptr<float>(h0), ptr<int64_t>(lengths),
+                                 dy.defined() ? &f->views[2 * form.gates] : nullptr, ptr<float>(dh), ptr<float>(dc),
+                                 ptr<void>(states), &f->views[form.gates], ptr<float>(dh0), ptr<void>(work),
+                                 stream_of<pt_scan_stream_t>(gates[0])));
+    variable_list out(kArgs);
+    out[6] = dh0;
+    if (gate_dim >= 0) {
+      out[7] = whole.defined() ? whole : at::cat(dgates, gate_dim);
+    } else {
+      for (int g = 0; g < form.gates; ++g) out[7 + g] = dgates[g];
+    }
+    return out;
+  }
+};
+
+// The gates as passed on, gate_dim (-1: one tensor per gate) and a gate's shape.
+struct Taken {
+  Gates xs;
+  int64_t gate_dim;
+  std::vector<int64_t> shape;
+};
+
+Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least) {
+  Taken t;
+  if (THPVariable_Check(x.ptr())) {
+    const Tensor v = THPVariable_Unpack(x.ptr());
+    TORCH_CHECK_VALUE(v.dim() > least, "stacked gates need at least ", least + 1, " dimensions, got ", v.sizes());
+    t.gate_dim = gate_dim < 0 ? gate_dim + v.dim() : gate_dim;
+    TORCH_CHECK_VALUE(t.gate_dim >= 0 && t.gate_dim < v.dim(), "gate_dim ", gate_dim, " is outside the tensor's ",
+                      v.dim(), " dimensions");
+    TORCH_CHECK_VALUE(v.size(t.gate_dim) % form.gates == 0, "dimension ", t.gate_dim, " holds ", form.gates,
+                      " gates, its size ", v.size(t.gate_dim), " is no multiple");
+    t.shape = v.sizes().vec();
+    t.shape[t.gate_dim] /= form.gates;
+    t.xs.push_back(v);
+  } else {
+    t.gate_dim = -1;
+    for (const py::handle& h : x) {
+      TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), "the gates must be tensors");
+      t.xs.push_back(THPVariable_Unpack(h.ptr()));
+    }
+    TORCH_CHECK_VALUE((int)t.xs.size() == form.gates, "the form takes ", form.gates, " gates, got ", t.xs.size());
+    t.shape = t.xs[0].sizes().vec();
+    for (const auto& v : t.xs)
+      TORCH_CHECK_VALUE((int64_t)t.shape.size() >= least && v.sizes() == t.xs[0].sizes(),
+                        "the gates need one shape of at least ", least, " dimensions");
+  }
+  const Tensor& v0 = t.xs[0];
+  for (const auto& v : t.xs) {
+    TORCH_CHECK_TYPE(v.layout() == at::kStrided && type_code(v.scalar_type()) >= 0, "gates of type ", v.scalar_type(),
+                     ": dense float32, bfloat16 or float16");
+    TORCH_CHECK_TYPE(v.scalar_type() == v0.scalar_type() && v.device() == v0.device(),
+                     "the gates must have one type and one device");
+  }
+  if (!v0.is_cuda()) raise(scan_error_type, "the gated scan runs on a ROCm device only (no CPU fallback)");
+  return t;
+}
+
+py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::string& form_name, int64_t dim,
+                     int64_t gate_dim, std::optional<Tensor> lengths, bool want_seq) {
+  const Form form = form_of(form_name);
+  Taken t = take(x, form, gate_dim, 2);
+  const int64_t nd = t.shape.size(), k = dim < 0 ? dim + nd : dim;
+  TORCH_CHECK_VALUE(k >= 0 && k < nd, "dim ", dim, " is outside the tensor's ", nd, " dimensions");
+  TORCH_CHECK_VALUE(k != t.gate_dim, "the gates cannot be stacked along the time dimension");
+  const auto device = t.xs[0].device();
+  const auto end = without(t.shape, k);
+  Tensor h, len;
+  if (h0) {
+    TORCH_CHECK_VALUE(h0->sizes() == at::IntArrayRef(end), "h0 has shape ", h0->sizes(), ", the state ",
+                      at::IntArrayRef(end));
+    TORCH_CHECK_TYPE(h0->device() == device && h0->is_floating_point(),
+                     "h0 must be a floating-point tensor on the gates' device");
+    h = h0->to(at::kFloat).contiguous();
+  }
+  if (lengths) {
+    TORCH_CHECK_VALUE(k != 0, "lengths need the batch in dimension 0, which is the time dimension here");
+    TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == t.shape[0], "lengths has shape ", lengths->sizes(),
+                      ", expected [", t.shape[0], "]");
+    TORCH_CHECK_TYPE(lengths->device() == device &&
+                         at::isIntegralType(lengths->scalar_type(), /*includeBool=*/false),
+                     "lengths must be an integer tensor on the gates' device");
+    len = lengths->to(at::kLong).contiguous();
+  }
+  auto give = [&](const Tensor& y, const Tensor& hl, const Tensor& cl) -> py::tuple {
+    py::object seq = want_seq ? py::cast(y) : py::none();
+    return form.lstm() ? py::make_tuple(seq, hl, cl) : py::make_tuple(seq, hl);
+  };
+  for (int64_t n : t.shape)
+    if (n == 0) {                        // no step or no column: nothing to launch
+      const Tensor zero = at::zeros(end, t.xs[0].options().dtype(at::kFloat).requires_grad(false));
+      const Tensor c = h.defined() ? h.clone() : zero;
+      Tensor y;
+      if (want_seq)
+        for (const auto& g : t.gate_dim >= 0 ? chunks(t.xs[0], form.gates, t.gate_dim) : t.xs)
+          y = y.defined() ? y + g : g.clone();
+      return form.lstm() ? give(y, zero.clone(), c) : give(y, c, Tensor());
+    }
+  int64_t back = -1;
+  if (k == nd - 1 && nd > 2 && t.shape[k] > 1 && t.shape[k - 1] > 1) {
+    // time innermost ([B, D, T]): a lane's steps would lie together and the
+    // lanes apart; two copies cost less than reading memory that way
+    Gates g = t.gate_dim >= 0 ? chunks(t.xs[0], form.gates, t.gate_dim) : t.xs;
+    for (auto& v : g) v = v.movedim(k, 1).contiguous();
+    t.xs = g;
+    t.gate_dim = -1;
+    back = k;
+  }
+  const int64_t at_dim = back >= 0 ? 1 : k;
+  bool grad = h.defined() && h.requires_grad();
+  for (const auto& v : t.xs) grad = grad || v.requires_grad();
+  Tensor y, hl, cl;
+  if (grad && at::GradMode::is_enabled()) {
+    std::optional<Tensor> a[4];
+    for (size_t g = 0; g < t.xs.size(); ++g) a[g] = t.xs[g];
+    auto opt = [](const Tensor& v) { return v.defined() ? std::optional<Tensor>(v) : std::nullopt; };
+    variable_list r = ScanFn::apply((int64_t)form.code, (int64_t)form.gates, at_dim, t.gate_dim, want_seq, opt(len),
+                                    opt(h), a[0], a[1], a[2], a[3]);
+    size_t i = 0;
+    if (want_seq) y = r[i++];
+    hl = r[i++];
+    if (form.lstm()) cl = r[i];
+  } else {
+    at::NoGradGuard no_grad;
+    Scanned r = forward(form, at_dim, t.gate_dim, want_seq, len, h, t.xs, false);
+    y = r.y;
+    hl = r.h_last;
+    cl = r.c_last;
+  }
+  if (back >= 0 && want_seq) y = y.movedim(1, back);
+  return give(y, hl, cl);
+}
+
+Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::string& form_name, int64_t gate_dim) {
+  const Form form = form_of(form_name);
+  Taken t = take(x, form, gate_dim, 1);
+  TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat && state.device() == t.xs[0].device(),
+                   "state must be a float32 tensor on the gates' device");
+  TORCH_CHECK_VALUE(state.sizes() == at::IntArrayRef(t.shape), "state has shape ", state.sizes(), ", expected ",
+                    at::IntArrayRef(t.shape));
+  if (at::GradMode::is_enabled()) {
+    bool grad = state.requires_grad();
+    for (const auto& v : t.xs) grad = grad || v.requires_grad();
+    if (grad)
+      raise(scan_error_type,
+            "gated_scan_step has no backward: call it under torch.no_grad(), or use gated_scan");
+  }
+  at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(state.device());
+  const Tensor y = at::empty(t.shape, t.xs[0].options().requires_grad(false));
+  if (y.numel() == 0) return y;
+  TORCH_CHECK_VALUE(disjoint(state.sizes(), state.strides()),
+                    "state's elements share memory: it cannot be updated in place");
+  Gates gates = t.gate_dim >= 0 ? chunks(t.xs[0], form.gates, t.gate_dim) : t.xs;
+  alike(gates);
+  Tensor s = state;
+  auto folded = [&] {
+    std::vector<const Tensor*> ts;
+    append(ts, gates);
+    ts.push_back(&s);
+    ts.push_back(&y);
+    return fold_of(ts, -1, false);
+  };
+  auto f = folded();
+  if (!f) {
+    for (auto& g : gates) g = g.contiguous();
+    s = state.contiguous();
+    f = folded();
+  }
+  const pt_scan_desc d{form.code, type_code(y.scalar_type()), f->b, f->c, 1, f->n};
+  check_scan(lib.scan_step(&d, f->views.data(), &f->views[form.gates], &f->views[form.gates + 1],
+                           stream_of<pt_scan_stream_t>(y)));
+  if (s.data_ptr() != state.data_ptr()) state.copy_(s);
+  return y;
+}
+
+// ------------------------------------------------------------------ clipping
+
+// Whether every element has a place of its own and the places are one run: the
+// order of the axes does not matter to a norm.
+bool dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
+
+void check_tensors(const std::vector<Tensor>& ts, const char* what) {
+  for (const auto& t : ts) {
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided && type_code(t.scalar_type()) >= 0, what, " of type ",
+                     t.scalar_type(), ": dense float32, bfloat16 or float16");
+    if (!t.is_cuda()) raise(clip_error_type, "clipping runs on a ROCm device only (no CPU fallback)");
+    if (t.device() != ts[0].device())
+      raise(clip_error_type, std::string(what) + " are on several devices: one process per GPU");
+  }
+}
+
+// The norm of `grads`; with max_norm >= 0 they are clipped, into `out` or in place.
+Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
+            const std::optional<std::vector<Tensor>>& out) {
+  int code = -1;
+  if (std::isinf(norm_type) && norm_type > 0) code = PT_CLIP_INF;
+  else if (norm_type == 1.0) code = PT_CLIP_L1;
+  else if (norm_type == 2.0) code = PT_CLIP_L2;
+  TORCH_CHECK_VALUE(code >= 0, "norm_type ", norm_type, ": 1, 2 or inf");
+  const bool scale = max_norm >= 0.0;
+  TORCH_CHECK_VALUE(!out || out->size() == grads.size(), out->size(), " outputs for ", grads.size(), " gradients");
+  check_tensors(grads, "gradients");
+  if (out) {
+    check_tensors(*out, "outputs");
+    for (size_t i = 0; i < grads.size(); ++i) {
+      const Tensor &g = grads[i], &o = (*out)[i];
+      TORCH_CHECK_VALUE(o.sizes() == g.sizes(), "an output of shape ", o.sizes(), " for a gradient of shape ",
+                        g.sizes());
+      TORCH_CHECK_TYPE(o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat, "an output of type ",
+                       o.scalar_type(), " for a gradient of type ", g.scalar_type());
+      if (o.device() != g.device()) raise(clip_error_type, "outputs are not on the gradients' device");
+      if (!disjoint(o.sizes(), o.strides()) && !dense(o))
+        raise(clip_error_type, "an output's elements share memory");
+    }
+  }
+  if (grads.empty()) return Tensor();
+  at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(grads[0].device());
+  std::vector<pt_clip_tensor> table(grads.size());
+  std::vector<Tensor> hold;                              // dense copies
+  std::vector<std::pair<Tensor, Tensor>> back;           // (tensor, dense copy): outputs to copy back
+  for (size_t i = 0; i < grads.size(); ++i) {
+    Tensor g = grads[i];
+    const Tensor& o = out ? (*out)[i] : grads[i];
+    const bool place = scale && (!out || o.is_same(g) ||
+                                 (o.data_ptr() == g.data_ptr() && o.scalar_type() == g.scalar_type() &&
+                                  o.strides() == g.strides()));
+    if (place && expanded(g))
+      raise(clip_error_type,
+            "a gradient's elements share memory (an expanded tensor): it cannot be clipped in place");
+    const bool copied = !dense(g);
+    if (copied) hold.push_back(g = g.contiguous());
+    pt_clip_tensor& e = table[i];
+    e.grad = g.data_ptr();
+    e.n = g.numel();
+    e.grad_type = type_code(g.scalar_type());
+    e.out = g.data_ptr();
+    e.out_type = e.grad_type;
+    if (!scale) continue;
+    if (place) {
+      if (copied) back.emplace_back(grads[i], g);
+    } else if (o.strides() == g.strides() && dense(o)) {
+      e.out = o.data_ptr();
+      e.out_type = type_code(o.scalar_type());
+    } else {                                             // another order of the axes: through a copy
+      Tensor d = at::empty_like(g, g.options().dtype(o.scalar_type()));
+      e.out = d.data_ptr();
+      e.out_type = type_code(o.scalar_type());
+      back.emplace_back(o, d);
+    }
+  }
+  const int64_t n = (int64_t)table.size();
+  const size_t size = lib.clip_work(table.data(), n);
+  if (!size) check_clip(PT_CLIP_ERR_ARG);
+  const Tensor work = bytes(size, grads[0]);
+  const Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  const auto stream = stream_of<pt_clip_stream_t>(grads[0]);
+  if (scale)
+    check_clip(lib.clip_grads(table.data(), n, code, max_norm, (float*)norm.data_ptr(), work.data_ptr(), stream));
+  else
+    check_clip(lib.clip_norm(table.data(), n, code, (float*)norm.data_ptr(), work.data_ptr(), stream));
+  for (auto& [o, d] : back) o.copy_(d);
+  return norm;
+}
+
+py::object py_fold(const std::vector<int64_t>& sizes, int64_t dim, const std::vector<std::vector<int64_t>>& strides,
+                   bool batch_first) {
+  std::vector<at::IntArrayRef> st(strides.begin(), strides.end());
+  const auto f = fold(sizes, dim, st, batch_first);
+  if (!f) return py::none();
+  py::list v;
+  for (const auto& s : f->views) v.append(py::make_tuple(s.sb, s.sc, s.st));
+  return py::make_tuple(f->b, f->c, f->n, v);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_native, m) {
+  m.def("open_scan", torch::wrap_pybind_function(open_scan));
+  m.def("open_clip", torch::wrap_pybind_function(open_clip));
+  m.def("gated_scan", torch::wrap_pybind_function(gated_scan));
+  m.def("gated_scan_step", torch::wrap_pybind_function(gated_scan_step));
+  m.def("clip", torch::wrap_pybind_function(clip));
+  m.def("fold", torch::wrap_pybind_function(py_fold));
+  m.def("disjoint", [](const std::vector<int64_t>& sizes, const std::vector<int64_t>& strides) {
+    return disjoint(sizes, strides);
+  });
+}

@@ -4,7 +4,8 @@ One compiler line per library (run in parallel): ``hipcc`` for the gfx950
 kernels — ``libptcell.so`` (InT / hGRU cell, include/pt_cell.h) and
 ``libptlstm.so`` (ConvLSTM cell, include/pt_lstm.h), ``libptscan.so`` (gated
 linear recurrences, include/pt_scan.h), ``libptclip.so`` (gradient norm and
-clipping, include/pt_clip.h) — and ``g++`` for the host
+clipping, include/pt_clip.h) — and ``g++`` for ``_native.so`` (the tensors' side
+of the last two: checks, layouts, autograd, on torch's C++ interface) and the host
 TFRecord reader ``libpttfr.so`` (include/pt_tfrecord.h, zlib).  They sit next
 to the ctypes bindings so they travel with the repository snapshot to the GPU
 box.  ``libptcell_diag.so`` is the same cell library built with -DPT_DIAG=1
@@ -46,6 +47,8 @@ LIBS = {
     "libptlstm_diag.so": _LSTM + (["-DPT_DIAG=1"],),
     "libptscan.so": ([os.path.join(CSRC, "pt_scan.hip")], [os.path.join(INC, "pt_scan.h")], _NO_PK),
     "libptclip.so": ([os.path.join(CSRC, "pt_clip.hip")], [os.path.join(INC, "pt_clip.h")], _NO_PK),
+    "_native.so": ([os.path.join(CSRC, "pt_torch.cpp")],
+                   [os.path.join(INC, "pt_scan.h"), os.path.join(INC, "pt_clip.h")]),
 }
 OUT = os.path.join(HERE, "libptcell.so")      # kept for callers of the old single-library API
 # The compiler line of the HIP libraries; part of the source stamp.
@@ -59,6 +62,22 @@ OUT = os.path.join(HERE, "libptcell.so")      # kept for callers of the old sing
 # with this flag in both the default and the -ffp-contract=on builds, never
 # without it).
 HIP_FLAGS = "--offload-arch=gfx950 -O3 -std=c++17 -fno-slp-vectorize"
+
+
+def _torch_flags():
+    """g++ flags of a Python module on torch's C++ interface (_native.so)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+    # the HIP headers want their platform named where the compiler is not hipcc
+    return (["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+            + [a for d in inc for a in ("-isystem", d)],
+            ["-L", os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ldl"])
 
 
 def _out(lib: str) -> str:
@@ -97,7 +116,11 @@ def build(force: bool = False, verbose: bool = True) -> str:
         if not force and up_to_date(lib):
             continue
         out = _out(lib)
-        if srcs[0].endswith(".cpp"):
+        if lib == "_native.so":
+            flags, libs = _torch_flags()
+            cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", INC,
+                   *flags, "-o", out + ".tmp", *srcs, *libs]
+        elif srcs[0].endswith(".cpp"):
             cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
                    "-pthread", "-Wall", "-I", INC, "-o", out + ".tmp", *srcs, "-lz", "-ldl"]
         else:

@@ -19,23 +19,18 @@ raise.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 import threading
 
-import torch
-from torch.autograd.function import once_differentiable
+import torch  # noqa: F401  (its libraries are what _native.so links against)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libptscan.so")
+NATIVE_PATH = os.path.join(HERE, "_native.so")
 
 # Exported symbols declared in include/pt_scan.h (tests check all are present).
 EXPORTS = ("pt_scan_backward", "pt_scan_forward", "pt_scan_last_error", "pt_scan_saved_bytes",
            "pt_scan_step", "pt_scan_version", "pt_scan_workspace_bytes")
-
-FORMS = {"leaky": 0, "lstm": 1}
-GATES = {"leaky": 2, "lstm": 4}
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 _P = ctypes.c_void_p
 _L = ctypes.c_int64
@@ -56,18 +51,15 @@ class PtScanError(RuntimeError):
 
 _lock = threading.RLock()
 _lib = None
+_native = None
 
 
 def load():
-    """Load (once) and return the library; raise if it is not built."""
+    """Load (once) and return the C ABI; raise if it is not built."""
     global _lib
-    if _lib is not None:
-        return _lib
     with _lock:
         if _lib is None:
-            if not os.path.exists(LIB_PATH):
-                raise PtScanError(f"{LIB_PATH} is missing: build the HIP extensions first "
-                                  "(python __graft_entry__.py build, or python -m ptamd.build)")
+            _require(LIB_PATH)
             lib = ctypes.CDLL(LIB_PATH)
             d, v = ctypes.POINTER(Desc), ctypes.POINTER(View)
             for name in ("pt_scan_saved_bytes", "pt_scan_workspace_bytes"):
@@ -82,236 +74,27 @@ def load():
     return _lib
 
 
-def _chk(lib, rc):
-    if rc != 0:
-        raise PtScanError(f"pt_scan error {rc}: {lib.pt_scan_last_error().decode(errors='replace')}")
+def _require(path):
+    if not os.path.exists(path):
+        raise PtScanError(f"{path} is missing: build the HIP extensions first "
+                          "(python __graft_entry__.py build, or python -m ptamd.build)")
 
 
-# ---------------------------------------------------------------- layouts
-
-def _merge(sizes, strides, lo, hi):
-    """(size, strides) of dimensions lo..hi-1 as one axis of every tensor, or
-    None; ``strides`` holds one tuple per tensor.  Axes of one element drop out."""
-    n, out = 1, None
-    for k in range(hi - 1, lo - 1, -1):
-        if sizes[k] == 1:
-            continue
-        if out is None:
-            out = [s[k] for s in strides]
-        elif any(s[k] != o * n for s, o in zip(strides, out)):
-            return None
-        n *= sizes[k]
-    return n, out or [0] * len(strides)
-
-
-@functools.lru_cache(maxsize=512)
-def _layout(sizes, dim, strides, batch_first):
-    """How tensors of ``sizes`` (their ``strides`` differing) fold into [batch]
-    [channels][steps][inner], time at ``dim`` (None: no time axis): (B, C, N,
-    [(sb, sc, st), ...]), or None where they do not.  ``batch_first``: the batch
-    is dimension 0 alone, as row ends need it."""
-    rest = [k for k in range(len(sizes)) if k != dim]
-    size = [sizes[k] for k in rest]
-    each = [tuple(s[k] for k in rest) for s in strides]
-    st = [0 if dim is None else s[dim] for s in strides]
-    first = 1 if batch_first else 0
-    # the inner axis: every trailing dimension that all tensors hold densely
-    inner, n = len(size), 1
-    while inner > first and all(size[inner - 1] == 1 or s[inner - 1] == n for s in each):
-        inner -= 1
-        n *= size[inner]
-    for cut in range(first, inner + 1):                # dimensions cut..inner-1: channels
-        b, c = _merge(size, each, 0, cut), _merge(size, each, cut, inner)
-        if b is not None and c is not None:
-            return b[0], c[0], n, list(zip(b[1], c[1], st))
-    return None
-
-
-class _Call:
-    """A shape's descriptor and buffer sizes (pure functions of the shape)."""
-
-    def __init__(self, form, dtype, b, c, t, n):
-        lib = load()
-        self.desc = Desc(FORMS[form], _TYPES[dtype], b, c, t, n)
-        self.ref = ctypes.byref(self.desc)
-        self.saved = lib.pt_scan_saved_bytes(self.ref)
-        self.work = lib.pt_scan_workspace_bytes(self.ref)
-
-
-@functools.lru_cache(maxsize=512)
-def _call(form, dtype, b, c, t, n):
-    return _Call(form, dtype, b, c, t, n)
-
-
-def _views(tensors, strides):
-    v = (View * len(tensors))()
-    for e, t, s in zip(v, tensors, strides):
-        e.data = t.data_ptr()
-        e.sb, e.sc, e.st = s
-    return v
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-class _on:
-    """The tensors' device as the current one, where it is not already."""
-
-    def __init__(self, device):
-        self.device = device
-        self.prev = None
-
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.device.index:
-            self.prev = cur
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
-        return False
-
-
-def _chunks(x, gates, gate_dim):
-    w = x.shape[gate_dim] // gates
-    return [x.narrow(gate_dim, g * w, w) for g in range(gates)]
-
-
-def _alike(gates):
-    """The gates with one set of strides, as the library reads them."""
-    st = gates[0].stride()
-    return gates if all(g.stride() == st for g in gates) else [g.contiguous() for g in gates]
-
-
-# ---------------------------------------------------------------- whole sequences
-
-def _fold(tensors, dim, ragged):
-    """The common layout of the tensors, or None."""
-    return _layout(tuple(tensors[0].shape), dim, tuple(t.stride() for t in tensors), ragged or dim != 0)
-
-
-def _forward(form, dim, gate_dim, want_seq, lengths, h0, xs, keep):
-    """(y, h_last, c_last, saved): the library's forward; ``keep`` for a backward."""
-    lib = load()
-    gates = _alike(_chunks(xs[0], GATES[form], gate_dim) if gate_dim is not None else list(xs))
-    x0 = gates[0]
-    shape, device = x0.shape, x0.device
-    seq = [torch.empty(shape, dtype=x0.dtype, device=device)] if want_seq else []
-    fold = _fold(gates + seq, dim, lengths is not None)
-    if fold is None:                         # no common layout: dense copies have one
-        gates = [g.contiguous() for g in gates]
-        fold = _fold(gates + seq, dim, lengths is not None)
-    b, c, n, strides = fold
-    call = _call(form, x0.dtype, b, c, shape[dim], n)
-    end = shape[:dim] + shape[dim + 1:]
-    h_last = torch.empty(end, device=device)
-    c_last = torch.empty(end, device=device) if form == "lstm" else None
-    saved = torch.empty(call.saved, dtype=torch.uint8, device=device) if keep and call.saved else None
-    work = torch.empty(call.work, dtype=torch.uint8, device=device) if call.work else None
-    with _on(device) as stream:
-        _chk(lib, lib.pt_scan_forward(call.ref, _views(gates, strides), _ptr(h0), _ptr(lengths),
-                                      _views(seq, strides[-1:]) if seq else None, h_last.data_ptr(),
-                                      _ptr(c_last), _ptr(saved), _ptr(work), stream))
-    return seq[0] if seq else None, h_last, c_last, saved
-
-
-class GatedScanFn(torch.autograd.Function):
-    """y, h_last, c_last = scan(gates; h0).  ``xs`` is one tensor with the gates
-    stacked along ``gate_dim`` or one tensor per gate (gate_dim None)."""
-
-    @staticmethod
-    def forward(ctx, form, dim, gate_dim, want_seq, lengths, h0, *xs):
-        y, h_last, c_last, saved = _forward(form, dim, gate_dim, want_seq, lengths, h0, xs, True)
-        ctx.save_for_backward(lengths, h0, saved, *xs)
-        ctx.args = (form, dim, gate_dim)
-        ctx.set_materialize_grads(False)
-        return y, h_last, c_last
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, d_h, d_c):
-        lib = load()
-        form, dim, gate_dim = ctx.args
-        lengths, h0, saved, *xs = ctx.saved_tensors
-        ragged = lengths is not None
-        need = ctx.needs_input_grad
-        if gate_dim is not None:
-            gates = _chunks(xs[0], GATES[form], gate_dim)
-            whole = torch.empty_like(xs[0])
-            dgates = _chunks(whole, GATES[form], gate_dim)
-        else:
-            gates = _alike(xs)
-            whole, dgates = None, [torch.empty_like(g) for g in gates]
-        if dy is not None and any(st == 0 and n > 1 for st, n in zip(dy.stride(), dy.shape)):
-            dy = dy.contiguous()             # an expanded dy (of a sum, a mean) has no dense axis
-        extra = [dy] if dy is not None else []
-        fold = _fold(gates + dgates + extra, dim, ragged)
-        if fold is None:
-            gates = [g.contiguous() for g in gates]
-            whole, dgates = None, [torch.empty_like(g) for g in gates]
-            extra = [dy.contiguous()] if dy is not None else []
-            fold = _fold(gates + dgates + extra, dim, ragged)
-        b, c, n, strides = fold
-        x0 = gates[0]
-        call = _call(form, x0.dtype, b, c, x0.shape[dim], n)
-        d_h = d_h.contiguous() if d_h is not None else None
-        d_c = d_c.contiguous() if d_c is not None else None
-        d_h0 = torch.empty_like(h0) if h0 is not None and need[5] else None
-        work = torch.empty(call.work, dtype=torch.uint8, device=x0.device) if call.work else None
-        k = len(gates)
-        xv, dv = _views(gates, strides[:k]), _views(dgates, strides[k:2 * k])
-        yv = _views(extra, strides[2 * k:]) if extra else None
-        with _on(x0.device) as stream:
-            _chk(lib, lib.pt_scan_backward(call.ref, xv, _ptr(h0), _ptr(lengths), yv, _ptr(d_h), _ptr(d_c),
-                                           _ptr(saved), dv, _ptr(d_h0), _ptr(work), stream))
-        if gate_dim is not None:
-            dxs = [whole if whole is not None else torch.cat(dgates, gate_dim)]
-        else:
-            dxs = dgates
-        return (None, None, None, None, None, d_h0, *[d if nd else None for d, nd in zip(dxs, need[6:])])
-
-
-def _gate_shape(x, form, gate_dim, least):
-    """(gates as passed on, gate_dim or None, a gate's shape) of a stacked tensor or a sequence of gates."""
-    g = GATES.get(form)
-    if g is None:
-        raise ValueError(f"unknown form {form!r}: one of {', '.join(FORMS)}")
-    if isinstance(x, torch.Tensor):
-        if x.dim() < least + 1:
-            raise ValueError(f"stacked gates need at least {least + 1} dimensions, got {tuple(x.shape)}")
-        k = gate_dim + x.dim() if gate_dim < 0 else gate_dim
-        if not 0 <= k < x.dim():
-            raise ValueError(f"gate_dim {gate_dim} is outside the tensor's {x.dim()} dimensions")
-        if x.shape[k] % g:
-            raise ValueError(f"{form}: dimension {k} holds {g} gates, its size {x.shape[k]} is no multiple")
-        shape = list(x.shape)
-        shape[k] //= g
-        xs = (x,)
-    else:
-        xs, k = tuple(x), None
-        if len(xs) != g:
-            raise ValueError(f"{form} takes {g} gates, got {len(xs)}")
-        if any(not isinstance(v, torch.Tensor) for v in xs):
-            raise TypeError("the gates must be tensors")
-        shape = list(xs[0].shape)
-        if len(shape) < least or any(list(v.shape) != shape for v in xs):
-            raise ValueError(f"the gates need one shape of at least {least} dimensions, "
-                             f"got {[tuple(v.shape) for v in xs]}")
-    x0 = xs[0]
-    if x0.dtype not in _TYPES:
-        raise TypeError(f"gates of type {x0.dtype}: float32, bfloat16 or float16")
-    if any(v.dtype != x0.dtype or v.device != x0.device for v in xs):
-        raise TypeError("the gates must have one type and one device")
-    if not x0.is_cuda:
-        raise PtScanError("the gated scan runs on a ROCm device only (no CPU fallback)")
-    return xs, k, tuple(shape)
+def native():
+    """The tensors' side (csrc/pt_torch.cpp) on top of the library."""
+    global _native
+    with _lock:
+        if _native is None:
+            _require(NATIVE_PATH)
+            _require(LIB_PATH)
+            from . import _native as mod
+            mod.open_scan(LIB_PATH, PtScanError)
+            _native = mod
+    return _native
 
 
 def gated_scan(x, h0=None, *, form="leaky", dim=1, gate_dim=2, lengths=None, want_seq=True):
-    """The recurrence over a whole sequence, differentiable in the gates and h0.
+    """The recurrence over a whole sequence, differentiable (once) in the gates and h0.
 
     x: the gates' pre-activations, stacked along ``gate_dim`` of one tensor
       ([B, T, G D] with the defaults; a Conv3d's [B, G C, T, H, W] has dim=2,
@@ -330,50 +113,8 @@ def gated_scan(x, h0=None, *, form="leaky", dim=1, gate_dim=2, lengths=None, wan
     gate's shape; h_last, f32, is y at each row's last step before its rounding
     (leaky: an empty row keeps h0; lstm: 0 there); c_last, f32, the last state.
     """
-    xs, gate_dim, shape = _gate_shape(x, form, gate_dim, 2)
-    nd = len(shape)
-    k = dim + nd if dim < 0 else dim
-    if not 0 <= k < nd:
-        raise ValueError(f"dim {dim} is outside the tensor's {nd} dimensions")
-    if k == gate_dim:
-        raise ValueError("the gates cannot be stacked along the time dimension")
-    device = xs[0].device
-    end = shape[:k] + shape[k + 1:]
-    if h0 is not None:
-        if tuple(h0.shape) != end:
-            raise ValueError(f"h0 has shape {tuple(h0.shape)}, the state {end}")
-        if h0.device != device or not h0.is_floating_point():
-            raise TypeError("h0 must be a floating-point tensor on the gates' device")
-        h0 = h0.float().contiguous()
-    if lengths is not None:
-        if k == 0:
-            raise ValueError("lengths need the batch in dimension 0, which is the time dimension here")
-        if tuple(lengths.shape) != (shape[0],):
-            raise ValueError(f"lengths has shape {tuple(lengths.shape)}, expected ({shape[0]},)")
-        if lengths.device != device or lengths.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
-            raise TypeError("lengths must be an integer tensor on the gates' device")
-        lengths = lengths.to(torch.int64).contiguous()
-    if 0 in shape:                               # no step or no column: nothing to launch
-        zero = torch.zeros(end, device=device)
-        h = zero if h0 is None else h0.clone()
-        y = sum(xs if gate_dim is None else _chunks(xs[0], GATES[form], gate_dim)) if want_seq else None
-        return (y, h) if form == "leaky" else (y, zero.clone(), h)
-    if k == nd - 1 and nd > 2 and shape[k] > 1 and shape[k - 1] > 1:
-        # time innermost ([B, D, T]): a lane's steps would lie together and the
-        # lanes apart; two copies cost less than reading memory that way
-        gates = xs if gate_dim is None else _chunks(xs[0], GATES[form], gate_dim)
-        res = gated_scan([g.movedim(k, 1).contiguous() for g in gates], h0, form=form, dim=1, lengths=lengths,
-                         want_seq=want_seq)
-        return (res[0].movedim(1, k) if want_seq else None, *res[1:])
-    args = (form, k, gate_dim, bool(want_seq), lengths, h0)
-    if torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in (h0, *xs)):
-        res = GatedScanFn.apply(*args, *xs)
-    else:
-        res = _forward(*args, xs, False)
-    return res[:2] if form == "leaky" else res[:3]
+    return (_native or native()).gated_scan(x, h0, form, dim, gate_dim, lengths, want_seq)
 
-
-# ---------------------------------------------------------------- one step
 
 def gated_scan_step(x, state, *, form="leaky", gate_dim=1):
     """One step of every row: ``state`` (f32, leaky: h, lstm: c) is updated in
@@ -384,43 +125,4 @@ def gated_scan_step(x, state, *, form="leaky", gate_dim=1):
       that do not overlap.  No gradients: a step that needs them is a
       ``gated_scan`` of one step.
     """
-    xs, gate_dim, shape = _gate_shape(x, form, gate_dim, 1)
-    if state.dtype != torch.float32 or state.device != xs[0].device:
-        raise TypeError("state must be a float32 tensor on the gates' device")
-    if tuple(state.shape) != shape:
-        raise ValueError(f"state has shape {tuple(state.shape)}, expected {shape}")
-    if torch.is_grad_enabled() and (state.requires_grad or any(v.requires_grad for v in xs)):
-        raise PtScanError("gated_scan_step has no backward: call it under torch.no_grad(), or use gated_scan")
-    y = torch.empty(shape, dtype=xs[0].dtype, device=state.device)
-    if y.numel() == 0:
-        return y
-    gates = _alike(_chunks(xs[0], GATES[form], gate_dim) if gate_dim is not None else list(xs))
-    if not _disjoint(shape, state.stride()):
-        raise ValueError("state's elements share memory: it cannot be updated in place")
-    fold = _layout(shape, None, tuple(t.stride() for t in (*gates, state, y)), False)
-    out = state
-    if fold is None:
-        gates = [g.contiguous() for g in gates]
-        out = state.contiguous()
-        fold = _layout(shape, None, tuple(t.stride() for t in (*gates, out, y)), False)
-    b, c, n, strides = fold
-    call = _call(form, y.dtype, b, c, 1, n)
-    lib = load()
-    v = _views([*gates, out, y], strides)
-    k = len(gates)
-    with _on(y.device) as stream:
-        _chk(lib, lib.pt_scan_step(call.ref, v, ctypes.byref(v[k]), ctypes.byref(v[k + 1]), stream))
-    if out is not state and out.data_ptr() != state.data_ptr():
-        state.copy_(out)
-    return y
-
-
-@functools.lru_cache(maxsize=512)
-def _disjoint(sizes, strides):
-    """Whether no two elements share memory, for strides that nest."""
-    reach = 1
-    for st, n in sorted((st, n) for st, n in zip(strides, sizes) if n > 1):
-        if st < reach:
-            return False
-        reach = st * (n - 1) + reach
-    return True
+    return (_native or native()).gated_scan_step(x, state, form, gate_dim)

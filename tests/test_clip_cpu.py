@@ -98,8 +98,3 @@ def test_python_refusals():
     p = torch.nn.Parameter(torch.zeros(3))                          # no gradient: left out
     assert float(clip.clip_grad_norm_([p], 1.0)) == 0.0
 
-
-def test_dense_layouts():
-    t = torch.empty(2, 3, 4)
-    assert clip._dense(t) and clip._dense(t.permute(2, 0, 1)) and clip._dense(torch.empty(0, 3))
-    assert not clip._dense(t[:, ::2]) and not clip._dense(t[..., :3]) and not clip._dense(torch.empty(1).expand(4))

@@ -78,7 +78,7 @@ def test_bad_pointers_are_refused():
     assert lib.pt_scan_step(r, good, odd, good, None) == 1 and b"aligned" in lib.pt_scan_last_error()
 
 
-def test_python_refusals():
+def test_refusals_of_tensors():
     x = torch.zeros(2, 5, 8)
     with pytest.raises(ValueError, match="form"):
         scan.gated_scan(x, form="gru")
@@ -136,7 +136,7 @@ def test_fold_addresses_every_element(shape, dim, perms, batch_first):
             t = torch.empty([shape[k] for k in p])
             tensors.append(t.permute([p.index(k) for k in range(len(shape))]))
     strides = tuple(t.stride() for t in tensors)
-    fold = scan._layout(tuple(shape), dim, strides, batch_first)
+    fold = scan.native().fold(shape, -1 if dim is None else dim, strides, batch_first)
     if fold is None:
         assert any(p is not None for p in perms)      # dense tensors of one order always fold
         return
@@ -152,11 +152,11 @@ def test_fold_refuses_what_it_cannot_address():
     # three separately strided groups in front of a dense axis
     t = torch.empty(2, 3, 4, 5, 6).permute(0, 2, 1, 3, 4)
     strided = torch.empty(4, 6, 8, 5, 6)[::2, ::2, ::2]
-    assert scan._layout((2, 3, 4, 5, 6), 3, (strided.stride(),), True) is None
-    assert scan._layout(tuple(t.shape), 3, (t.stride(),), True) is None
+    assert scan.native().fold((2, 3, 4, 5, 6), 3, (strided.stride(),), True) is None
+    assert scan.native().fold(t.shape, 3, (t.stride(),), True) is None
 
 
 def test_overlapping_states_are_seen():
-    assert scan._disjoint((4, 6), (6, 1)) and scan._disjoint((4, 6), (1, 4)) and scan._disjoint((1, 6), (0, 1))
-    assert scan._disjoint((4, 6), (100, 2))
-    assert not scan._disjoint((4, 6), (0, 1)) and not scan._disjoint((4, 6), (3, 1))
+    apart = scan.native().disjoint
+    assert apart((4, 6), (6, 1)) and apart((4, 6), (1, 4)) and apart((1, 6), (0, 1)) and apart((4, 6), (100, 2))
+    assert not apart((4, 6), (0, 1)) and not apart((4, 6), (3, 1))
