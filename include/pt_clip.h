@@ -2,7 +2,7 @@
  * pt_clip.h — C ABI of the gradient norm and clipping (gfx950, libptclip.so).
  *
  * The reference's clip_grad_norm_ (utils/misc_functions.py:48-69) over a list
- * of tensors of any sizes and types in two launches for each TABLE of them:
+ * of tensors of any sizes and types, in two launches for every 192 to 320 of them:
  *   N = (sum over all elements |g|^p)^(1/p)  (p = 1, 2; inf: the largest |g|)
  *   k = min(1, max_norm / (N + 1e-6)),  out = k g
  * Sums are held in 64 bits, so that squares of f32 neither overflow nor
@@ -46,7 +46,7 @@ size_t pt_clip_workspace_bytes(const pt_clip_tensor* t, int64_t count);
 int pt_clip_norm(const pt_clip_tensor* t, int64_t count, int norm_type, float* norm, void* workspace,
                  pt_clip_stream_t stream);
 
-/* norm = N, out = k grad.  In place and k = 1, a tensor is not touched.
+/* norm = N, out = k grad.  All in place and k = 1, no tensor is touched.
  * Refused: an out that overlaps another tensor, or its own grad other than
  * exactly; max_norm below 0 or NaN. */
 int pt_clip_grads(const pt_clip_tensor* t, int64_t count, int norm_type, double max_norm, float* norm,

@@ -2,12 +2,12 @@
 //
 // Bound by memory: the norm reads every gradient once, the scaling reads it
 // again and writes it.  The tensors' pointers travel in the kernel arguments
-// (TABLE of them a launch: no copy to the device, nothing to keep alive), a
-// tensor is cut into chunks of CHUNK elements, and a workgroup takes chunks
-// id, id + grid, ...  Every workgroup leaves one 64-bit partial; the scaling's
-// workgroups each add all partials themselves, in the same order, which costs
-// less than a launch between the two.  The scaling walks the chunks from the
-// last to the first: what the norm read last is still in the card's cache.
+// (4 KB a launch: no copy to the device, nothing to keep alive), a tensor is cut
+// into chunks of CHUNK elements, and a workgroup takes chunks id, id + grid, ...
+// Every workgroup leaves one 64-bit partial; the scaling's workgroups each add
+// all partials themselves, in the same order, which costs less than a launch
+// between the two.  The scaling walks the chunks from the last to the first:
+// what the norm read last is still in the card's cache.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -33,23 +33,27 @@ int fail(int code, const char* msg) {
 }
 
 constexpr int NT = 256;               // threads of a workgroup
-constexpr int VEC = 8;                // elements of a thread at a time: 16 or 32 bytes
-constexpr int UNROLL = 4;
-constexpr int CHUNK = NT * VEC * UNROLL;
-constexpr int TABLE = 96;             // tensors of a launch: 36 bytes each, under the 4 KB of arguments
+constexpr int CHUNK = 8192;           // elements of a tensor that a workgroup takes at a time
 constexpr int GRID = 1024;            // workgroups of a launch at most: 4 a compute unit
 constexpr int64_t INLINE_PARTS = 4096;   // partials that every workgroup adds by itself
+constexpr int64_t PIECE = (int64_t)1 << 28;   // elements of a table entry; larger tensors take several
 
-struct Table {
-  const void* in[TABLE];
-  void* out[TABLE];
-  int64_t n[TABLE];
-  uint32_t first[TABLE + 1];          // first chunk of each tensor
-  uint8_t in_type[TABLE], out_type[TABLE];
+// A launch's tensors, as many as 4 KB of kernel arguments hold: 12 bytes each
+// where outputs are the gradients themselves (or there are none), else 20.
+template <bool OUT> struct Table {
+  static constexpr int MAX = OUT ? 192 : 320;
+  const void* in[MAX];
+  void* out[OUT ? MAX : 1];
+  uint32_t n[MAX];                    // elements << 2 in 30 bits, type in the low two
+  uint32_t out_f32[OUT ? MAX / 32 : 1];   // bit: the output is f32, whatever the gradient
   int count;
 };
+static_assert(sizeof(Table<false>) <= 3960 && sizeof(Table<true>) <= 3960, "kernel arguments of 4 KB");
 
-template <typename T> using vecu = T __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+// V elements in one access, at any alignment of their own.  A lane moves 16 bytes
+// of the wider side at a time, so that a wave's access is one run of 1 KB (32
+// bytes a lane leave every other 16 to the next access).
+template <typename T, int V> using vecu = T __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 
 // Two partial results joined; a NaN stays.
 template <int P> __device__ __forceinline__ double join(double a, double b) {
@@ -77,41 +81,76 @@ template <int P> __device__ double block_join(double v, double* red) {
   return v;
 }
 
-// The tensor that chunk id belongs to (uniform over the workgroup).
-__device__ __forceinline__ int tensor_of(const Table& t, uint32_t id) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.first[mid] <= id) lo = mid; else hi = mid - 1;
+// First chunk of every tensor of the table, and the chunks of all (at [count]),
+// in shared memory: a running sum by the first wave.
+template <typename Tab> __device__ __forceinline__ void first_chunks(const Tab& t, uint32_t* first) {
+  if (threadIdx.x < 64) {
+    uint32_t base = 0;
+    for (int k0 = 0; k0 < t.count; k0 += 64) {
+      const int k = k0 + threadIdx.x;
+      const uint32_t c = k < t.count ? ((t.n[k] >> 2) + CHUNK - 1) / CHUNK : 0;
+      uint32_t s = c;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(s, o);
+        if ((int)threadIdx.x >= o) s += v;
+      }
+      if (k < t.count) first[k] = base + s - c;
+      base += __shfl(s, 63);
+    }
+    if (threadIdx.x == 0) first[t.count] = base;
   }
-  return lo;
+  __syncthreads();
 }
 
-template <int P, typename T> __device__ __forceinline__ double chunk_norm(const T* p, int64_t n, double acc) {
-  if (n >= CHUNK) {
-    vecu<T> v[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) v[u] = *(const vecu<T>*)(p + (u * NT + threadIdx.x) * VEC);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) acc = term<P>(acc, (float)v[u][k]);
-  } else {
-    for (int i = threadIdx.x; i < (int)n; i += NT) acc = term<P>(acc, (float)p[i]);
+// The tensor that chunk id belongs to (uniform over the workgroup).
+__device__ __forceinline__ int tensor_of(const uint32_t* first, int count, uint32_t id) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= id) lo = mid; else hi = mid - 1;
   }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+template <int P, typename T> __device__ __forceinline__ double chunk_norm(const T* p, uint32_t n, double acc) {
+  constexpr int V = 16 / sizeof(T), U = CHUNK / (NT * V);
+  vecu<T, V> v[U];
+  if (n >= CHUNK) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *(const vecu<T, V>*)(p + (u * NT + threadIdx.x) * V);
+  } else {                               // a tensor's end: one thread has a part of its V elements
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = (u * NT + threadIdx.x) * V;
+      v[u] = (T)0.f;
+      if (i + V <= n) {
+        v[u] = *(const vecu<T, V>*)(p + i);
+      } else if (i < n) {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (i + k < n) v[u][k] = p[i + k];
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc = term<P>(acc, (float)v[u][k]);
   return acc;
 }
 
-template <int P> __global__ __launch_bounds__(NT) void k_norm(Table t, double* part) {
+template <int P> __global__ __launch_bounds__(NT) void k_norm(Table<false> t, double* part) {
   __shared__ double red[NT / 64];
+  __shared__ uint32_t first[Table<false>::MAX + 1];
+  first_chunks(t, first);
   double acc = 0.0;
-  const uint32_t total = t.first[t.count];
+  const uint32_t total = first[t.count];
   for (uint32_t id = blockIdx.x; id < total; id += gridDim.x) {
-    const int k = tensor_of(t, id);
-    const int64_t at = (int64_t)(id - t.first[k]) * CHUNK;
-    const int64_t n = t.n[k] - at;
-    if (t.in_type[k] == PT_CLIP_F32) acc = chunk_norm<P>((const float*)t.in[k] + at, n, acc);
-    else if (t.in_type[k] == PT_CLIP_BF16) acc = chunk_norm<P>((const __bf16*)t.in[k] + at, n, acc);
+    const int k = tensor_of(first, t.count, id);
+    const uint32_t at = (id - first[k]) * CHUNK, n = (t.n[k] >> 2) - at, type = t.n[k] & 3;
+    if (type == PT_CLIP_F32) acc = chunk_norm<P>((const float*)t.in[k] + at, n, acc);
+    else if (type == PT_CLIP_BF16) acc = chunk_norm<P>((const __bf16*)t.in[k] + at, n, acc);
     else acc = chunk_norm<P>((const _Float16*)t.in[k] + at, n, acc);
   }
   acc = block_join<P>(acc, red);
@@ -136,47 +175,66 @@ template <int P> __global__ __launch_bounds__(NT) void k_total(const double* par
 }
 
 template <typename T, typename O>
-__device__ __forceinline__ void chunk_scale(const T* p, O* o, int64_t n, double k) {
+__device__ __forceinline__ void chunk_scale(const T* p, O* o, uint32_t n, double k) {
+  constexpr int V = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O)), U = CHUNK / (NT * V);
+  auto times = [k](T x) { return (O)(float)((double)(float)x * k); };
   if (n >= CHUNK) {
-    vecu<T> v[UNROLL];
+    vecu<T, V> v[U];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) v[u] = *(const vecu<T>*)(p + (u * NT + threadIdx.x) * VEC);
+    for (int u = 0; u < U; ++u) v[u] = *(const vecu<T, V>*)(p + (u * NT + threadIdx.x) * V);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      vecu<O> r;
+    for (int u = 0; u < U; ++u) {
+      vecu<O, V> r;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) r[j] = (O)(float)((double)(float)v[u][j] * k);
-      *(vecu<O>*)(o + (u * NT + threadIdx.x) * VEC) = r;
+      for (int j = 0; j < V; ++j) r[j] = times(v[u][j]);
+      *(vecu<O, V>*)(o + (u * NT + threadIdx.x) * V) = r;
     }
   } else {
-    for (int i = threadIdx.x; i < (int)n; i += NT) o[i] = (O)(float)((double)(float)p[i] * k);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = (u * NT + threadIdx.x) * V;
+      if (i + V <= n) {
+        const vecu<T, V> v = *(const vecu<T, V>*)(p + i);
+        vecu<O, V> r;
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = times(v[j]);
+        *(vecu<O, V>*)(o + i) = r;
+      } else if (i < n) {
+        for (uint32_t j = i; j < n; ++j) o[j] = times(p[j]);
+      }
+    }
   }
 }
 
-template <int P>
-__global__ __launch_bounds__(NT) void k_scale(Table t, const double* part, int64_t parts, double max_norm, float* norm) {
+template <int P, bool OUT>
+__global__ __launch_bounds__(NT) void k_scale(Table<OUT> t, const double* part, int64_t parts, double max_norm,
+                                              float* norm) {
   __shared__ double red[NT / 64];
+  __shared__ uint32_t first[Table<OUT>::MAX + 1];
   const double n = root<P>(total_of<P>(part, parts, red));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const double q = max_norm / (n + 1e-6);
+  if (!OUT && q >= 1.0) return;                          // k = 1 in place: nothing changes
   // The product is taken in 64 bits and rounded once: k is far below f32's range
   // when the norm is far above it.  (A NaN goes through.)
   const double k = q >= 1.0 ? 1.0 : q;
-  const uint32_t total = t.first[t.count];
+  first_chunks(t, first);
+  const uint32_t total = first[t.count];
   for (uint32_t r = blockIdx.x; r < total; r += gridDim.x) {
     const uint32_t id = total - 1 - r;
-    const int i = tensor_of(t, id);
-    if (q >= 1.0 && t.out[i] == t.in[i]) continue;       // k = 1 in place: nothing changes
-    const int64_t at = (int64_t)(id - t.first[i]) * CHUNK;
-    const int64_t left = t.n[i] - at;
-    if (t.in_type[i] == PT_CLIP_F32) {
-      chunk_scale((const float*)t.in[i] + at, (float*)t.out[i] + at, left, k);
-    } else if (t.in_type[i] == PT_CLIP_BF16) {
-      if (t.out_type[i] == PT_CLIP_F32) chunk_scale((const __bf16*)t.in[i] + at, (float*)t.out[i] + at, left, k);
-      else chunk_scale((const __bf16*)t.in[i] + at, (__bf16*)t.out[i] + at, left, k);
+    const int i = tensor_of(first, t.count, id);
+    const uint32_t at = (id - first[i]) * CHUNK, left = (t.n[i] >> 2) - at, type = t.n[i] & 3;
+    const void* p = t.in[i];
+    void* o = OUT ? t.out[OUT ? i : 0] : (void*)p;
+    const bool wide = OUT && (t.out_f32[OUT ? i / 32 : 0] >> (i % 32) & 1);
+    if (type == PT_CLIP_F32) {
+      chunk_scale((const float*)p + at, (float*)o + at, left, k);
+    } else if (type == PT_CLIP_BF16) {
+      if (wide) chunk_scale((const __bf16*)p + at, (float*)o + at, left, k);
+      else chunk_scale((const __bf16*)p + at, (__bf16*)o + at, left, k);
     } else {
-      if (t.out_type[i] == PT_CLIP_F32) chunk_scale((const _Float16*)t.in[i] + at, (float*)t.out[i] + at, left, k);
-      else chunk_scale((const _Float16*)t.in[i] + at, (_Float16*)t.out[i] + at, left, k);
+      if (wide) chunk_scale((const _Float16*)p + at, (float*)o + at, left, k);
+      else chunk_scale((const _Float16*)p + at, (_Float16*)o + at, left, k);
     }
   }
 }
@@ -185,30 +243,36 @@ __global__ __launch_bounds__(NT) void k_scale(Table t, const double* part, int64
 
 int size_of(int type) { return type == PT_CLIP_F32 ? 4 : 2; }
 
-// The next launch's tensors, from t[at]: fills `tab`, returns where the one after starts.
-int64_t next_table(const pt_clip_tensor* t, int64_t count, int64_t at, Table& tab) {
+// Where a walk over the tensors stands: tensor, and element in it.
+struct At {
+  int64_t i = 0, e = 0;
+};
+
+// The next launch's tensors from `at` on, which moves behind them: their chunks.
+template <bool OUT> uint32_t next_table(const pt_clip_tensor* t, int64_t count, At& at, Table<OUT>& tab) {
+  uint32_t chunks = 0;
   tab.count = 0;
-  uint64_t chunks = 0;
-  for (; at < count && tab.count < TABLE; ++at) {
-    if (t[at].n == 0) continue;
-    const uint64_t c = (uint64_t)((t[at].n + CHUNK - 1) / CHUNK);
-    if (chunks + c > 0xfff00000u) break;                 // (the grid's stride may not wrap)
-    const int k = tab.count++;
-    tab.in[k] = t[at].grad;
-    tab.out[k] = t[at].out;
-    tab.n[k] = t[at].n;
-    tab.in_type[k] = (uint8_t)t[at].grad_type;
-    tab.out_type[k] = (uint8_t)t[at].out_type;
-    tab.first[k] = (uint32_t)chunks;
-    chunks += c;
+  if (OUT) std::fill(std::begin(tab.out_f32), std::end(tab.out_f32), 0u);
+  while (at.i < count && tab.count < Table<OUT>::MAX) {
+    const pt_clip_tensor& x = t[at.i];
+    const int64_t n = std::min(x.n - at.e, PIECE);
+    if (n > 0) {
+      const int k = tab.count++;
+      tab.in[k] = (const char*)x.grad + at.e * size_of(x.grad_type);
+      tab.n[k] = (uint32_t)n << 2 | (uint32_t)x.grad_type;
+      if (OUT) {
+        tab.out[OUT ? k : 0] = (char*)x.out + at.e * size_of(x.out_type);
+        if (x.out_type == PT_CLIP_F32) tab.out_f32[OUT ? k / 32 : 0] |= 1u << (k % 32);
+      }
+      chunks += (uint32_t)((n + CHUNK - 1) / CHUNK);
+      at.e += n;
+    }
+    if (at.e >= x.n) at = At{at.i + 1, 0};
   }
-  tab.first[tab.count] = (uint32_t)chunks;
-  return at;
+  return chunks;
 }
 
-unsigned grid_of(const Table& tab) {
-  return std::min<uint32_t>(tab.first[tab.count], GRID);
-}
+unsigned grid_of(uint32_t chunks) { return std::min<uint32_t>(chunks, GRID); }
 
 int check(const pt_clip_tensor* t, int64_t count, bool out) {
   if (count < 0 || (count > 0 && !t)) return fail(PT_CLIP_ERR_ARG, "clip: null tensor list");
@@ -255,25 +319,38 @@ int check_overlap(const pt_clip_tensor* t, int64_t count) {
 }
 
 int64_t parts_of(const pt_clip_tensor* t, int64_t count) {
-  Table tab;
-  int64_t parts = 0, at = 0;
-  while (at < count) {
-    at = next_table(t, count, at, tab);
-    parts += grid_of(tab);
-  }
+  Table<false> tab;
+  int64_t parts = 0;
+  for (At at; at.i < count;) parts += grid_of(next_table(t, count, at, tab));
   return parts;
+}
+
+// The scaling's launches, from the last tensors to the first.
+template <int P, bool OUT>
+void scale_all(const pt_clip_tensor* t, int64_t count, const double* part, int64_t parts, double max_norm, float* norm,
+               hipStream_t s) {
+  Table<OUT> tab;
+  std::vector<At> starts;
+  for (At at; at.i < count;) {
+    starts.push_back(at);
+    next_table(t, count, at, tab);
+  }
+  for (size_t k = starts.size(); k-- > 0;) {
+    At at = starts[k];
+    const unsigned g = grid_of(next_table(t, count, at, tab));
+    if (!g) continue;
+    hipLaunchKernelGGL((k_scale<P, OUT>), dim3(g), dim3(NT), 0, s, tab, part, parts, max_norm, norm);
+    norm = nullptr;                                      // written once
+  }
 }
 
 template <int P>
 int run(const pt_clip_tensor* t, int64_t count, bool scale, double max_norm, float* norm, double* part,
         hipStream_t s) {
-  Table tab;
+  Table<false> tab;
   int64_t parts = 0;
-  std::vector<int64_t> starts;
-  for (int64_t at = 0; at < count;) {
-    starts.push_back(at);
-    at = next_table(t, count, at, tab);
-    const unsigned g = grid_of(tab);
+  for (At at; at.i < count;) {
+    const unsigned g = grid_of(next_table(t, count, at, tab));
     if (g) hipLaunchKernelGGL((k_norm<P>), dim3(g), dim3(NT), 0, s, tab, part + parts);
     parts += g;
   }
@@ -285,14 +362,12 @@ int run(const pt_clip_tensor* t, int64_t count, bool scale, double max_norm, flo
     n = 1;
     norm = nullptr;
   }
-  if (scale)
-    for (size_t k = starts.size(); k-- > 0;) {
-      next_table(t, count, starts[k], tab);
-      const unsigned g = grid_of(tab);
-      if (!g) continue;
-      hipLaunchKernelGGL((k_scale<P>), dim3(g), dim3(NT), 0, s, tab, from, n, max_norm, norm);
-      norm = nullptr;
-    }
+  if (scale && parts) {
+    bool place = true;
+    for (int64_t i = 0; i < count; ++i) place = place && (t[i].n == 0 || t[i].out == t[i].grad);
+    if (place) scale_all<P, false>(t, count, from, n, max_norm, norm, s);
+    else scale_all<P, true>(t, count, from, n, max_norm, norm, s);
+  }
   return hipGetLastError() == hipSuccess ? 0 : fail(PT_CLIP_ERR_HIP, "clip: launch failed");
 }
 

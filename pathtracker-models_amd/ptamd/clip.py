@@ -1,7 +1,7 @@
 """The global gradient norm and clipping (include/pt_clip.h, ``libptclip.so``).
 
 The reference's ``clip_grad_norm_`` (utils/misc_functions.py:48-69) over any
-number of tensors in two launches for every 96 of them, with sums in 64 bits
+number of tensors in two launches for every 192 to 320 of them, with sums in 64 bits
 and a fixed order of addition, so that data-parallel ranks that hold the same
 averaged gradients clip them by the same factor bit for bit.  The norm stays on
 the device: nothing here synchronises, unless ``error_if_nonfinite`` asks.
