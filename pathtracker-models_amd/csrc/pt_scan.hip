@@ -73,19 +73,26 @@ struct Args {
 
 template <typename T, int V> using vec = T __attribute__((ext_vector_type(V)));
 
-// e^-x for x >= 0.  ACC (f32 data): the product x log2(e) is carried in two
+// A constant in a scalar register: as a literal it would need the short encoding,
+// which takes no |x| or -x of its operand, at one more instruction a use.
+__device__ __forceinline__ float in_scalar(float c) {
+  asm("" : "+s"(c));
+  return c;
+}
+
+// e^-Nx for x >= 0, N a power of two.  ACC (f32 data): the product x log2(e) is carried in two
 // parts, which keeps the error at an ulp for large x too; for 16-bit data the
 // single product's error (x 2^-24 relative) is far below the data's step.
-template <bool ACC> __device__ __forceinline__ float exp_minus(float x) {
-  constexpr float L2E = 1.44269502f, L2E_LO = 1.92596303e-8f, LN2 = 0.693147182f;
+template <bool ACC, int N = 1> __device__ __forceinline__ float exp_minus(float x) {
+  constexpr float L2E = N * 1.44269502f, L2E_LO = N * 1.92596303e-8f, LN2 = 0.693147182f;
   if constexpr (ACC) {
     x = x > 104.f ? 104.f : x;                 // (inf would make the low part NaN; NaN stays)
-    const float t = x * L2E;
-    const float lo = __builtin_fmaf(x, L2E_LO, __builtin_fmaf(x, L2E, -t));
+    const float c = in_scalar(L2E), t = x * c;
+    const float lo = __builtin_fmaf(x, L2E_LO, __builtin_fmaf(x, c, -t));
     const float r = __builtin_amdgcn_exp2f(-t);
     return __builtin_fmaf(r, -lo * LN2, r);
   } else {
-    return __builtin_amdgcn_exp2f(-x * L2E);
+    return __builtin_amdgcn_exp2f(x * in_scalar(-L2E));
   }
 }
 
@@ -108,7 +115,7 @@ template <bool ACC> __device__ __forceinline__ Logistic logistic(float x) {
 // odd series below 0.35 (next term 2e-9 relative), where 1 - e would cancel.
 template <bool ACC> __device__ __forceinline__ float tanh_d(float x, float& d) {
   const float ax = __builtin_fabsf(x);
-  const float e = exp_minus<ACC>(2.f * ax), r = recip<ACC>(1.f + e);
+  const float e = exp_minus<ACC, 2>(ax), r = recip<ACC>(1.f + e);
   d = 4.f * e * r * r;
   float t = __builtin_copysignf((1.f - e) * r, x);
   if constexpr (ACC) {
@@ -226,6 +233,28 @@ __device__ __forceinline__ void store_steps(const T (&r)[L], char* p, int64_t st
   }
 }
 
+// Registers whose contents no longer matter (else a loop that loads them in one
+// branch copies the old contents in the other).
+template <typename T, int L> __device__ __forceinline__ void forget(T (&r)[L]) {
+#pragma unroll
+  for (int l = 0; l < L; ++l) asm("" : "=v"(r[l]));
+}
+
+// Values that are to be there at this point: what was loaded for them is free for
+// the next loads, and a rare branch that makes them is not turned into selects.
+template <int L> __device__ __forceinline__ void settle(float (&r)[L]) {
+#pragma unroll
+  for (int l = 0; l < L; ++l) asm volatile("" : "+v"(r[l]));
+}
+
+// An element as f32 in a register of its own (seen through, |x| of a 16-bit
+// element becomes integer arithmetic instead of a modifier of the next operand).
+template <typename T> __device__ __forceinline__ float as_f32(T x) {
+  float f = (float)x;
+  if constexpr (sizeof(T) == 2) asm("" : "+v"(f));
+  return f;
+}
+
 template <int FORM> constexpr int gates_of() { return FORM == PT_SCAN_LEAKY ? 2 : 4; }
 // Steps of one wave in a chunk of the backward, as many as stay in 128
 // registers; the forward keeps less per step and takes twice as many.
@@ -293,6 +322,7 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
     for (int g = 0; g < GA; ++g) load_steps(raw[g], xp[g], a.xs.t, xo, lim - t0);
     if constexpr (!AGG && FORM == PT_SCAN_LSTM)         // o is wanted for y, or at the row's last step
       if (seq || (t0 < w.end && w.end - t0 <= L)) load_steps(raw[3], xp[3], a.xs.t, xo, lim - t0);
+      else forget(raw[3]);
 #pragma unroll
     for (int g = 0; g < G; ++g) xp[g] += x_step;
   };
@@ -307,18 +337,33 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
       yp += a.ys.t * CH;
       continue;
     }
-    float A[L], B[L];
-    T o[L];
+    float A[L], B[L], O[L];
+    const bool out_here = seq || (FORM == PT_SCAN_LSTM && !AGG && t0 < w.end && w.end - t0 <= L);
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
-      coefs<FORM, T>((float)raw[0][l], (float)raw[1][l], GA > 2 ? (float)raw[GA - 1][l] : 0.f, A[l], B[l]);
-      if constexpr (!AGG && FORM == PT_SCAN_LSTM) o[l] = raw[3][l];
+    for (int l = 0; l < L; ++l)
+      coefs<FORM, T>(as_f32(raw[0][l]), as_f32(raw[1][l]), GA > 2 ? as_f32(raw[GA - 1][l]) : 0.f, A[l], B[l]);
+    if constexpr (!AGG && FORM == PT_SCAN_LSTM) {
+      if (out_here) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) O[l] = logistic<ACC>(as_f32(raw[3][l])).s;
+      } else {
+        forget(O);
+      }
     }
-    if (t + CH < lim) fetch(t0 + CH);
+    settle(A);
+    settle(B);
+    if (t + CH < lim) {
+      fetch(t0 + CH);
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) forget(raw[g]);
+    }
     if (live < L) {                                     // behind the row's end the state stays
 #pragma unroll
       for (int l = 0; l < L; ++l)
         if (l >= live) { A[l] = 1.f; B[l] = 0.f; }
+      settle(A);
+      settle(B);
     }
 
     float cin = carry;
@@ -348,14 +393,13 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
     for (int l = 0; l < L; ++l) B[l] = cin = __builtin_fmaf(A[l], cin, B[l]);   // the states
     if constexpr (W == 1) carry = cin;
     if constexpr (FORM == PT_SCAN_LSTM) {
-      const bool has_last = t0 < w.end && w.end - t0 <= L;
-      if (seq || has_last) {
+      if (out_here) {
 #pragma unroll
         for (int l = 0; l < L; ++l) {
           float d;
-          B[l] = logistic<ACC>((float)o[l]).s * tanh_d<ACC>(B[l], d);
+          B[l] = O[l] * tanh_d<ACC>(B[l], d);
         }
-        if (has_last && a.h_last && w.on) {
+        if (a.h_last && t0 < w.end && w.end - t0 <= L && w.on) {
 #pragma unroll
           for (int l = 0; l < L; ++l)
             if (t0 + l == w.end - 1) a.h_last[w.state] = B[l];
@@ -436,6 +480,7 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
     for (int g = 0; g < (LEAKY ? AGG ? 1 : 2 : 3); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, live);
     if constexpr (!LEAKY)
       if (enters(t0)) load_steps(raw[3], xp[3], a.xs.t, xo, live);
+      else forget(raw[3]);
     if (has_dy) load_steps(rdy, yp, a.ys.t, yo, live);
     if constexpr (!(AGG && LEAKY)) {
       const float* s = tc > 0 ? a.saved + (tc / CH - 1) * a.cols_all : a.h0;
@@ -465,32 +510,59 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
     const int t0 = t + w.wave * L, live = lim - t0;
     // a; what the gradients are made of; dy, then dL/dh_t through y_t
     float A[L], K0[L], K1[L], D[L];
-    float B[L], K2[L];                                  // lstm
-    T o[L];
+    float B[L], K2[L], O[L], OP[L];                     // lstm
     float cin = nst;
 #pragma unroll
     for (int l = 0; l < L; ++l) {
       D[l] = (float)rdy[l];
       if constexpr (LEAKY) {
-        const Logistic z = logistic<ACC>((float)raw[0][l]);
+        const Logistic z = logistic<ACC>(as_f32(raw[0][l]));
         A[l] = z.sm;
         if constexpr (!AGG) {
           K1[l] = z.s;
-          K0[l] = (float)raw[1][l];
+          K0[l] = as_f32(raw[1][l]);
         }
       } else {
-        const Logistic f = logistic<ACC>((float)raw[1][l]), i = logistic<ACC>((float)raw[0][l]);
+        const Logistic f = logistic<ACC>(as_f32(raw[1][l])), i = logistic<ACC>(as_f32(raw[0][l]));
         float d;
-        const float th = tanh_d<ACC>((float)raw[2][l], d);
+        const float th = tanh_d<ACC>(as_f32(raw[2][l]), d);
         A[l] = f.s;
         B[l] = i.s * th;
         K0[l] = i.p * th;
         K1[l] = f.p;
         K2[l] = i.s * d;
-        o[l] = raw[3][l];
       }
     }
-    if (t > t_beg) fetch(t - CH);
+    if constexpr (!LEAKY) {
+      if (enters(t0)) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+          const Logistic g = logistic<ACC>(as_f32(raw[3][l]));
+          O[l] = g.s;
+          OP[l] = g.p;
+        }
+      } else {
+        forget(O);
+        forget(OP);
+      }
+    }
+    settle(A);
+    settle(D);
+    if constexpr (!(LEAKY && AGG)) {
+      settle(K0);
+      settle(K1);
+    }
+    if constexpr (!LEAKY) {
+      settle(B);
+      settle(K2);
+    }
+    if (t > t_beg) {
+      fetch(t - CH);
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) forget(raw[g]);
+      if (has_dy) forget(rdy);
+    }
     if (live < L) {                                     // behind the row's end: h' = h, dx = 0
 #pragma unroll
       for (int l = 0; l < L; ++l)
@@ -499,6 +571,9 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
           if constexpr (!LEAKY) B[l] = 0.f;
           else if constexpr (!AGG) K1[l] = 0.f;
         }
+      settle(A);
+      if constexpr (!LEAKY) settle(B);
+      else if constexpr (!AGG) settle(K1);
     }
 
     float gin = carry;
@@ -545,16 +620,16 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
           const float e = a.d_h_last[w.state];
 #pragma unroll
           for (int l = 0; l < L; ++l) D[l] += t0 + l == w.end - 1 ? e : 0.f;
+          settle(D);
         }
 #pragma unroll
         for (int l = 0; l < L; ++l) {
           K1[l] *= cin;
           cin = __builtin_fmaf(A[l], cin, B[l]);
-          const Logistic g = logistic<ACC>((float)o[l]);
           float d;
           const float th = tanh_d<ACC>(cin, d);
-          out[l] = (T)(D[l] * th * g.p);
-          D[l] *= g.s * d;
+          out[l] = (T)(D[l] * th * OP[l]);
+          D[l] *= O[l] * d;
         }
       } else {
 #pragma unroll
