@@ -3,7 +3,7 @@
 
 Same flags (utils/opts.py), same per-batch semantics as the reference loop
 (mainclean.py:169-256): prepare_data -> model_step -> BCEWithLogits ->
-acc_scores -> backward -> Adam step -> zero_grad, per-epoch train/val ``.npz``
+acc_scores -> backward -> [--clip-grad] -> Adam step -> zero_grad, per-epoch train/val ``.npz``
 logs, a 4-batch validation (``logiters=3``, :238), EarlyStopping on the
 validation accuracy (patience 200, :125) that ends the run.
 
@@ -38,7 +38,7 @@ import torch.distributed as dist  # noqa: E402
 from ptamd.dist import CellDist, GradBucket, env_rank, lockstep  # noqa: E402
 from utils import engine  # noqa: E402
 from utils.earlystopping import EarlyStopping  # noqa: E402
-from utils.misc_functions import AverageMeter, acc_scores  # noqa: E402
+from utils.misc_functions import AverageMeter, acc_scores, clip_grad_norm_  # noqa: E402
 from utils.opts import parser  # noqa: E402
 from utils.TFRDataset import tfr_data_loader  # noqa: E402
 
@@ -187,6 +187,8 @@ def main(argv=None):
     val_log_dict = {'loss': [], 'balacc': [], 'precision': [], 'recall': [], 'f1score': []}
     train_log_dict = {'loss': [], 'balacc': [], 'precision': [], 'recall': [], 'f1score': [],
                       'jvpen': [], 'scaled_loss': []}
+    if args.clip_grad > 0:
+        train_log_dict['gradnorm'] = []     # before clipping, one a step
     stopped = False
     for epoch in range(args.start_epoch, args.epochs):
         batch_time, data_time, losses = AverageMeter(), AverageMeter(), AverageMeter()
@@ -217,6 +219,9 @@ def main(argv=None):
 
             loss.backward()
             bucket.allreduce_mean()
+            if args.clip_grad > 0:          # averaged gradients: every rank clips by the same factor
+                norm = clip_grad_norm_(model.parameters(), args.clip_grad)
+                train_log_dict['gradnorm'].append(norm.item())
             optimizer.step()
             optimizer.zero_grad()
             batch_time.update(time.perf_counter() - end)

@@ -39,6 +39,7 @@ from torch.nn import init
 
 from ptamd import lstm
 from ptamd import readout as ro
+from ptamd import scan
 from ptamd.cell import target_channel
 from ptamd.lstm import run_steps
 
@@ -268,10 +269,18 @@ class ConvLSTMVideo(nn.Module):
     attention maps there, is the per-frame hidden state h_t here (the
     reference ConvLSTM's testmode collects exactly those, convlstm.py:127-135;
     the cell has no attention gate).
+
+    ``lesion_hidden=True`` (registry name ``convlstm_no_hidden``) cuts the
+    hidden-to-gate convolutions Wh, as InT's ``no_inh`` and ``lesion_*`` cut
+    theirs: the gates see the frame alone, so the k x k convolutions of all
+    frames run as one batch and the state is scanned over time
+    (ptamd.scan.gated_scan) instead of walked.  The parameters and their keys
+    stay; Wh is frozen.  d h_T / d h_{T-1} is 0 then, and jv_penalty the
+    constant that InT returns (InT.py:243).
     """
 
     def __init__(self, dimensions=25, timesteps=8, kernel_size=7, jacobian_penalty=False,
-                 grad_method='bptt', nl=F.softplus):
+                 grad_method='bptt', nl=F.softplus, lesion_hidden=False):
         super().__init__()
         if grad_method != 'bptt':
             raise NotImplementedError("ConvLSTMVideo trains with BPTT only")
@@ -289,6 +298,10 @@ class ConvLSTMVideo(nn.Module):
         self.target_conv = nn.Conv2d(2, 1, 5, padding=2)
         init.zeros_(self.target_conv.bias)
         self.readout_dense = nn.Linear(1, 1)
+        self.lesion_hidden = lesion_hidden
+        if lesion_hidden:
+            for g in ("i", "f", "c", "o"):
+                getattr(self.unit1, f"Wh{g}").requires_grad_(False)
 
     @property
     def cell_dtype(self):
@@ -297,6 +310,19 @@ class ConvLSTMVideo(nn.Module):
     @cell_dtype.setter
     def cell_dtype(self, v):
         self.unit1.cell_dtype = v
+
+    def _scan_frames(self, x, want_seq):
+        """(h_T [B,C,H,W], h_1..T [B,T,C,H,W] or None) without the hidden
+        convolutions: gates of every frame [B,T,4C,H,W], then the scan over T."""
+        frames = lstm.stem(x, self.preproc.weight, self.preproc.bias).transpose(1, 2)
+        b, t, c, h, w = frames.shape
+        dtype = torch.bfloat16 if self.cell_dtype == 'bf16' else torch.float32
+        ws = self.unit1.cell_weights()
+        gates = F.conv2d(frames.reshape(b * t, c, h, w).to(dtype), torch.cat(ws[:4]).to(dtype),
+                         torch.cat(ws[4:8]).to(dtype), padding=self.unit1.padding)
+        seq, h_t, _ = scan.gated_scan(gates.view(b, t, -1, h, w), form='lstm', dim=1, gate_dim=2,
+                                      want_seq=want_seq)
+        return h_t, seq
 
     # forward also takes the raw u8 clips [B,T,H,W,3] (engine.prepare_data
     # keep_u8): the stem kernel converts them exactly as prepare_data would
@@ -307,11 +333,15 @@ class ConvLSTMVideo(nn.Module):
         # per-step input (pt_lstm_forward_stem; r05: the f32 stem output and its
         # layout conversions, ~3 ms of a 45 ms step, no longer exist)
         steps = x.shape[1] if x.dtype == torch.uint8 else x.shape[2]
-        want_jv = self.training and steps >= 2
+        want_jv = self.training and steps >= 2 and not self.lesion_hidden
         lstm._require_device(x)
-        res = lstm.stem_steps(x, self.preproc.weight, self.preproc.bias, self.unit1.cell_weights(),
-                              ksize=self.kernel_size, dtype=self.cell_dtype, want_jv=want_jv,
-                              want_seq=testmode)
+        if self.lesion_hidden:
+            h_t, hidden = self._scan_frames(x, testmode)
+            res = h_t, None, None, hidden.float().transpose(1, 2) if testmode else None
+        else:
+            res = lstm.stem_steps(x, self.preproc.weight, self.preproc.bias, self.unit1.cell_weights(),
+                                  ksize=self.kernel_size, dtype=self.cell_dtype, want_jv=want_jv,
+                                  want_seq=testmode)
         h_t, jv = res[0], res[2]
         out = ro.readout(h_t, target_channel(x), self.readout_conv, self.target_conv,
                          self.readout_dense)                         # ptamd/readout.py

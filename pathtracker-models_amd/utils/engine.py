@@ -88,6 +88,10 @@ def model_selector(args, timesteps, device, fb_kernel_size=7, dimensions=32):
     if args.model == 'convlstm':                 # ConvLSTM on the clips
         return convlstm.ConvLSTMVideo(dimensions=25, timesteps=timesteps,
                                       kernel_size=fb_kernel_size, grad_method='bptt')
+    if args.model == 'convlstm_no_hidden':       # its gates see the frame alone: a scan over time
+        return convlstm.ConvLSTMVideo(dimensions=25, timesteps=timesteps,
+                                      kernel_size=fb_kernel_size, grad_method='bptt',
+                                      lesion_hidden=True)
     if args.model == 'ffhgru':
         return ffhgru_hierarchy.FFhGRU(dimensions=dimensions, timesteps=timesteps,
                                        kernel_size=fb_kernel_size, jacobian_penalty=False,

@@ -7,8 +7,11 @@ hard ``.cuda()``: everything stays on the logits' device.
   precision= tp / max(#pred, 1e-6)  (:19-24)
   recall   = tp / B                 (:18,22 — P is the batch size, not #positives)
   f1       = 2 tp / (B + #pred)     (:26)
+  clip_grad_norm_          (:48-69) on the device: ptamd/clip.py
 """
 import torch
+
+from ptamd.clip import clip_grad_norm_  # noqa: F401
 
 
 def metric_scores(target, pred):

@@ -8,6 +8,9 @@ running without the reference's cluster paths (all optional):
                       TFRecord shards under --data-root first (no dataset offline)
   --results-root DIR  results folder root (reference: hard-coded /cifs/..., mainclean.py:124)
   --max-iters N       stop each epoch after N batches (smoke runs)
+and one for the reference's clip_grad_norm_ (utils/misc_functions.py:48-69, which
+its own loop leaves uncalled):
+  --clip-grad MAX     scale the gradients to a norm of at most MAX before each step
 """
 import argparse
 
@@ -58,6 +61,9 @@ parser.add_argument('--data-root', type=str, default=None)
 parser.add_argument('--synthetic', type=int, default=0)
 parser.add_argument('--results-root', type=str, default=None)
 parser.add_argument('--max-iters', type=int, default=0)
+parser.add_argument('--clip-grad', type=float, default=0.0, metavar='MAX',
+                    help='largest global gradient norm (L2, all parameters together, after the '
+                         'averaging over the ranks); 0: no clipping (default)')
 parser.add_argument('--f32-input', default=False, action='store_true',
                     help='hand the HIP-cell models the f32 [B,3,T,H,W] tensor instead of the raw u8 clips')
 parser.add_argument('--sync-bn', default=False, action='store_true',
