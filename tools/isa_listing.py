@@ -24,8 +24,10 @@ BTARGET = re.compile(r"<(\S+)\+0x([0-9a-f]+)>\s*$")
 def disassemble(so_path: str) -> str:
     with tempfile.TemporaryDirectory() as d:
         fb, co = os.path.join(d, "fb.bin"), os.path.join(d, "co.o")
-        subprocess.run(["objcopy", "--dump-section", f".hip_fatbin={fb}", so_path], check=True,
-                       capture_output=True)
+        # with an output of its own: objcopy otherwise rewrites the library in place,
+        # under the mapping of a process that has it loaded
+        subprocess.run(["objcopy", "--dump-section", f".hip_fatbin={fb}", so_path,
+                        os.path.join(d, "copy.so")], check=True, capture_output=True)
         subprocess.run([f"{LLVM}/clang-offload-bundler", "--unbundle", "--type=o", f"--targets={TARGET}",
                         f"--input={fb}", f"--output={co}"], check=True, capture_output=True)
         return subprocess.run([f"{LLVM}/llvm-objdump", "-d", "--mcpu=gfx950", co], check=True,
