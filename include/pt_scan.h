@@ -19,7 +19,7 @@
  * Conventions as pt_cell.h: caller-allocated device buffers, explicit stream,
  * 0 or PT_SCAN_ERR_* with a thread-local message, no state between calls.  No
  * call synchronises; every call can be captured into a graph.  Results do not
- * depend on timing: there are no atomics.
+ * depend on timing: two runs agree bit for bit.
  */
 #ifndef PT_SCAN_H
 #define PT_SCAN_H
@@ -56,7 +56,8 @@ typedef struct pt_scan_view {
 
 /* Bytes of `saved`, the states that the backward starts its pieces from. */
 size_t pt_scan_saved_bytes(const pt_scan_desc* d);
-/* Bytes of the scratch of one call (forward and backward alike); may be 0. */
+/* Bytes of the scratch of one call (forward and backward alike); may be 0.  Its
+ * contents do not matter, and calls that may run at once need one each. */
 size_t pt_scan_workspace_bytes(const pt_scan_desc* d);
 
 /* x: one view per gate.  h0: the state before the first step, or NULL (zeros).

@@ -14,10 +14,13 @@
 // Layout.  A lane owns a column (channel, inner), so every load of a wave is 64
 // neighbouring elements of one step.  Two 16-bit columns a lane would halve the
 // loads, but what a step keeps until its gradient is known then passes 128
-// registers: the backward spilled and took 3.1 times as long.  Where the columns do
-// not fill the card the time axis is also cut over workgroups (`segs`): a
-// first launch reduces each segment to (P, q), and the second starts each
-// segment from the composition of those before it.
+// registers: the backward spilled and took 3.1 times as long.
+//
+// Where the columns do not fill the card the time axis is also cut over
+// workgroups, a chunk each (the chain): a workgroup reduces its chunk to (P, q)
+// as above, publishes the pair, takes the pairs of the chunks before its own
+// and finishes its chunk from its registers.  The pairs are always joined in
+// the same order, so the results do not depend on timing.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -40,8 +43,14 @@ int fail(int code, const char* msg) {
   return code;
 }
 
-constexpr int MAX_SEGS = 64;
-constexpr int SPLIT_W = 8;       // waves of a workgroup when the time axis is cut over workgroups
+// Waves of a workgroup of the chain.  A longer chunk pays the joining less often,
+// two workgroups a compute unit hide it better: 32 tiles of 16384 steps, leaky
+// bf16, forward 72 us with 8 waves and 64 with 16, backward 93 and 99.
+constexpr int CHAIN_FWD = 16, CHAIN_BWD = 8;
+constexpr int GROUP = 32;        // chunks after which the chain hands a state on, so that joins stay short
+static_assert(GROUP % CHAIN_FWD == 0 && GROUP % CHAIN_BWD == 0 && (GROUP & (GROUP - 1)) == 0,
+              "a join is shared out evenly over the waves");
+static_assert(CHAIN_FWD == 2 * CHAIN_BWD, "the forward's chunks are two of the backward's, as without the chain");
 
 // One kind of sequence tensor (all gates share their strides): strides in bytes.
 struct Strides {
@@ -61,14 +70,15 @@ struct Args {
   const float* d_c_last;
   float* d_h0;
   float* saved;            // [chunk of the backward][B][C N]: the state before it (the first: h0)
-  float* agg;              // [segment][B][C N] pairs (P, q)
+  uint32_t* ticket;        // the chain: the next workgroup's number
+  uint64_t* pairs;         // the chain: [chunk][B][C N] published pairs (P, q)
+  uint64_t* states;        // the chain: [group][B][C N] published pairs (1, state)
   int64_t cols_all;        // B C N
   int64_t C, N;
   int64_t cg, groups;      // channels per column group, groups per batch row
   int64_t outer;           // B groups
   int T;                   // steps
-  int seg_steps;           // a multiple of the chunk
-  int tiles, segs;
+  int tiles, segs;         // column tiles of a row; chunks of the chain
 };
 
 template <typename T, int V> using vec = T __attribute__((ext_vector_type(V)));
@@ -161,7 +171,7 @@ __device__ __forceinline__ int here(int k) {
 }
 template <typename T> using gval = __attribute__((address_space(1))) T;
 
-// Where a workgroup works: column tile, row, segment; and a lane's column.
+// Where a workgroup works: column tile, row, chunk of the chain; and a lane's column.
 struct Where {
   int seg, lane, wave, end;  // `end`: the batch row's
   int64_t b, c0;             // batch row; the group's first channel
@@ -169,10 +179,9 @@ struct Where {
   int64_t state;             // this lane's column in [B][C][N]
   uint32_t off_c, off_n;     // channel in the group, position in the inner axis
 
-  __device__ __forceinline__ Where(const Args& a) {
+  __device__ __forceinline__ Where(const Args& a, uint32_t id) {    // the host keeps the grid below 2^31
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t id = blockIdx.x;            // the host keeps the grid below 2^31
     const uint32_t tile = id % (uint32_t)a.tiles;
     id /= (uint32_t)a.tiles;
     const uint32_t o = id % (uint32_t)a.outer;
@@ -251,98 +260,42 @@ template <int L> __device__ __forceinline__ void settle(float (&r)[L]) {
 // element becomes integer arithmetic instead of a modifier of the next operand).
 template <typename T> __device__ __forceinline__ float as_f32(T x) {
   float f = (float)x;
-  if constexpr (sizeof(T) == 2) asm("" : "+v"(f));
+  asm("" : "+v"(f));
   return f;
 }
 
 template <int FORM> constexpr int gates_of() { return FORM == PT_SCAN_LEAKY ? 2 : 4; }
-// Steps of one wave in a chunk of the backward, as many as stay in 128
-// registers; the forward keeps less per step and takes twice as many.
+// Steps of one wave in a chunk of the backward, as many as stay in 128 registers
+// beside the next chunk's loads; the forward keeps less per step and takes twice
+// as many.  In the chain a chunk is alone and has the registers of two.
 template <int FORM> constexpr int back_steps() { return FORM == PT_SCAN_LEAKY ? 8 : 4; }
+template <int FORM> constexpr int chain_steps() { return FORM == PT_SCAN_LEAKY ? 16 : 8; }
 
 using f32x2 = vec<float, 2>;
 
-// The state before segment `seg`.
-__device__ __forceinline__ float start_state(const Args& a, const Where& w) {
-  float c = a.h0 ? a.h0[w.state] : 0.f;
-  const f32x2* p = (const f32x2*)a.agg + w.state;
-  for (int s = 0; s < w.seg; ++s) {
-    const f32x2 e = p[s * a.cols_all];
-    c = __builtin_fmaf(e[0], c, e[1]);
-  }
-  return c;
-}
+// ------------------------------------------------------------------ a wave's steps, forward
 
-// a and b of one element of the forward.
-template <int FORM, typename T>
-__device__ __forceinline__ void coefs(float g0, float g1, float g2, float& a, float& b) {
-  constexpr bool ACC = sizeof(T) == 4;
-  const Logistic l = logistic<ACC>(g0);
-  if constexpr (FORM == PT_SCAN_LEAKY) {
-    a = l.sm;
-    b = l.s * g1;
-  } else {
-    float d;
-    a = logistic<ACC>(g1).s;
-    b = l.s * tanh_d<ACC>(g2, d);
-  }
-}
+template <int FORM, typename T, int L> struct Fwd {
+  static constexpr int G = gates_of<FORM>();
+  static constexpr bool LSTM = FORM == PT_SCAN_LSTM, ACC = sizeof(T) == 4;
+  float A[L], B[L], O[L];        // a; b, then the states, then y; lstm: s(o)
 
-// Forward.  AGG: reduce a segment to (P, q) only.
-template <int FORM, typename T, int W, bool AGG>
-__global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
-  static_assert(W > 1 || !AGG, "one wave never splits the time axis over workgroups");
-  constexpr int G = gates_of<FORM>(), L = 2 * back_steps<FORM>(), CH = W * L;
-  constexpr int GA = FORM == PT_SCAN_LEAKY ? 2 : 3;      // the gates that make a and b
-  constexpr bool ACC = sizeof(T) == 4;
-  // The waves' (P, q).  Two sets, used in turn: a wave writes a set again only
-  // behind a barrier that every wave reaches after its last read of it, so one
-  // barrier a chunk does.
-  __shared__ f32x2 pq[2][W][64];
-  const Where w(a);
-  const int t_beg = w.seg * a.seg_steps;
-  const int t_end = a.T - t_beg < a.seg_steps ? a.T : t_beg + a.seg_steps;
-  const int lim = w.end < t_end ? w.end : t_end;
-  const bool seq = !AGG && a.y != nullptr;
-
-  float carry = AGG ? 0.f : start_state(a, w), prod = 1.f;
-
-  const int mine = t_beg + w.wave * L;                  // this wave's first step
-  const int64_t x_at = w.base(a.xs, mine), x_step = a.xs.t * CH;
-  const uint32_t xo = w.lane_off(a.xs, sizeof(T));
-  const char* xp[G];
+  // From what was loaded.  out_here: some y is made of these steps.
+  __device__ __forceinline__ void make(const T (&raw)[G][L], bool out_here) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) xp[g] = a.x[g] + x_at;
-  char* yp = seq ? a.y + w.base(a.ys, mine) : nullptr;
-  const uint32_t yo = seq ? w.lane_off(a.ys, sizeof(T)) : 0;
-
-  T raw[G][L];
-  auto fetch = [&](int t0) {
-#pragma unroll
-    for (int g = 0; g < GA; ++g) load_steps(raw[g], xp[g], a.xs.t, xo, lim - t0);
-    if constexpr (!AGG && FORM == PT_SCAN_LSTM)         // o is wanted for y, or at the row's last step
-      if (seq || (t0 < w.end && w.end - t0 <= L)) load_steps(raw[3], xp[3], a.xs.t, xo, lim - t0);
-      else forget(raw[3]);
-#pragma unroll
-    for (int g = 0; g < G; ++g) xp[g] += x_step;
-  };
-  fetch(mine);
-
-  int par = 0;
-  for (int t = t_beg; t < t_end; t += CH) {
-    const int t0 = t + w.wave * L, live = lim - t0;
-    if (t >= lim) {                                     // the whole chunk is behind the row's end
-      if (!seq) break;
-      if (w.on) store_steps(raw[0], yp, a.ys.t, yo, 0, t_end - t0);
-      yp += a.ys.t * CH;
-      continue;
+    for (int l = 0; l < L; ++l) {
+      const Logistic g = logistic<ACC>(as_f32(raw[0][l]));
+      if constexpr (!LSTM) {
+        A[l] = g.sm;
+        B[l] = g.s * as_f32(raw[1][l]);
+      } else {
+        float d;
+        A[l] = logistic<ACC>(as_f32(raw[1][l])).s;
+        B[l] = g.s * tanh_d<ACC>(as_f32(raw[2][l]), d);
+      }
+      asm volatile("" : "+v"(A[l]), "+v"(B[l]));        // (one after the other, not all at once)
     }
-    float A[L], B[L], O[L];
-    const bool out_here = seq || (FORM == PT_SCAN_LSTM && !AGG && t0 < w.end && w.end - t0 <= L);
-#pragma unroll
-    for (int l = 0; l < L; ++l)
-      coefs<FORM, T>(as_f32(raw[0][l]), as_f32(raw[1][l]), GA > 2 ? as_f32(raw[GA - 1][l]) : 0.f, A[l], B[l]);
-    if constexpr (!AGG && FORM == PT_SCAN_LSTM) {
+    if constexpr (LSTM) {
       if (out_here) {
 #pragma unroll
         for (int l = 0; l < L; ++l) O[l] = logistic<ACC>(as_f32(raw[3][l])).s;
@@ -352,47 +305,28 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
     }
     settle(A);
     settle(B);
-    if (t + CH < lim) {
-      fetch(t0 + CH);
-    } else {
+  }
+  // Behind the row's end the state stays.
+  __device__ __forceinline__ void end_row(int live) {
+    if (live >= L) return;
 #pragma unroll
-      for (int g = 0; g < G; ++g) forget(raw[g]);
-    }
-    if (live < L) {                                     // behind the row's end the state stays
+    for (int l = 0; l < L; ++l)
+      if (l >= live) { A[l] = 1.f; B[l] = 0.f; }
+    settle(A);
+    settle(B);
+  }
+  __device__ __forceinline__ f32x2 piece() const {
+    f32x2 e = {A[0], B[0]};
 #pragma unroll
-      for (int l = 0; l < L; ++l)
-        if (l >= live) { A[l] = 1.f; B[l] = 0.f; }
-      settle(A);
-      settle(B);
-    }
-
-    float cin = carry;
-    if constexpr (W > 1) {
-      f32x2 own = {A[0], B[0]};
+    for (int l = 1; l < L; ++l) e = f32x2{e[0] * A[l], __builtin_fmaf(A[l], e[1], B[l])};
+    return e;
+  }
+  // The steps from state c on: y and h_last are written, the state after them returned.
+  __device__ __forceinline__ float finish(const Args& a, const Where& w, float c, int t0, int live, int room, bool seq,
+                                          bool out_here, char* yp, uint32_t yo) {
 #pragma unroll
-      for (int l = 1; l < L; ++l) own = f32x2{own[0] * A[l], __builtin_fmaf(A[l], own[1], B[l])};
-      pq[par][w.wave][w.lane] = own;
-      lds_barrier();
-      // compose: the state before this wave's steps, and the one after the chunk
-      const int wave = here(w.wave);
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const f32x2 e = pq[par][k][w.lane];
-        cin = k == wave ? carry : cin;
-        carry = __builtin_fmaf(e[0], carry, e[1]);
-        if constexpr (AGG) prod *= e[0];
-      }
-      par ^= 1;
-      if constexpr (!AGG)                               // where the backward's chunks begin
-        if (a.saved && (w.wave == 0 || w.wave == W / 2) && t0 > 0 && t0 < a.T && w.on)
-          a.saved[(t0 / (CH / 2) - 1) * a.cols_all + w.state] = cin;
-    }
-    if constexpr (AGG) continue;
-
-#pragma unroll
-    for (int l = 0; l < L; ++l) B[l] = cin = __builtin_fmaf(A[l], cin, B[l]);   // the states
-    if constexpr (W == 1) carry = cin;
-    if constexpr (FORM == PT_SCAN_LSTM) {
+    for (int l = 0; l < L; ++l) B[l] = c = __builtin_fmaf(A[l], c, B[l]);
+    if constexpr (LSTM) {
       if (out_here) {
 #pragma unroll
         for (int l = 0; l < L; ++l) {
@@ -410,118 +344,118 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
       T out[L];
 #pragma unroll
       for (int l = 0; l < L; ++l) out[l] = (T)B[l];
-      if (w.on) store_steps(out, yp, a.ys.t, yo, live, t_end - t0);
-      yp += a.ys.t * CH;
+      if (w.on) store_steps(out, yp, a.ys.t, yo, live, room);
     }
+    return c;
   }
+};
 
-  if (w.wave != 0 || !w.on) return;
-  if constexpr (AGG) {
-    ((f32x2*)a.agg)[w.seg * a.cols_all + w.state] = f32x2{prod, carry};
-  } else if (w.seg == a.segs - 1) {
-    if (a.c_last) a.c_last[w.state] = carry;
-    if (a.h_last && FORM == PT_SCAN_LEAKY) a.h_last[w.state] = carry;
-    if (a.h_last && FORM == PT_SCAN_LSTM && w.end == 0) a.h_last[w.state] = 0.f;
-  }
+// The states after a row's last step (lstm: h_last comes with that step's y, and
+// is 0 for a row without one).
+template <int FORM> __device__ __forceinline__ void last_states(const Args& a, const Where& w, float c) {
+  if (!w.on) return;
+  if (a.c_last) a.c_last[w.state] = c;
+  if (a.h_last && FORM == PT_SCAN_LEAKY) a.h_last[w.state] = c;
+  if (a.h_last && FORM == PT_SCAN_LSTM && w.end == 0) a.h_last[w.state] = 0.f;
 }
 
-// Backward.  AGG: reduce a segment, from zero at its far end, to (P, q) of the
-// gradient that leaves it towards the past.
-template <int FORM, typename T, int W, bool AGG>
-__global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
-  static_assert(W > 1 || !AGG, "one wave never splits the time axis over workgroups");
-  constexpr int G = gates_of<FORM>(), L = back_steps<FORM>(), CH = W * L;
-  constexpr bool LEAKY = FORM == PT_SCAN_LEAKY, ACC = sizeof(T) == 4;
-  __shared__ f32x2 pq[2][W][64];              // forward (P, q); two sets in turn, as in the forward
-  __shared__ float gq[2][W][64];              // backward q (its P is the same)
-  const Where w(a);
-  const int seg = AGG ? w.seg + 1 : w.seg;    // nothing is behind segment 0
-  const int t_beg = seg * a.seg_steps;
-  const int t_end = a.T - t_beg < a.seg_steps ? a.T : t_beg + a.seg_steps;
-  const int lim = w.end < t_end ? w.end : t_end;
-  const bool has_dy = a.y != nullptr;
-  // lstm: whether any gradient enters through y among the L steps from t0 (without
-  // a dy it does at the row's last step alone, and o, tanh(c) matter only there)
-  auto enters = [&](int t0) { return has_dy || (a.d_h_last && t0 < w.end && w.end - t0 <= L); };
+// Forward, a workgroup walking a column tile's whole row.
+template <int FORM, typename T, int W>
+__global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
+  constexpr int G = gates_of<FORM>(), L = 2 * back_steps<FORM>(), CH = W * L;
+  constexpr bool LSTM = FORM == PT_SCAN_LSTM;
+  // The waves' (P, q).  Two sets, used in turn: a wave writes a set again only
+  // behind a barrier that every wave reaches after its last read of it, so one
+  // barrier a chunk does.
+  __shared__ f32x2 pq[2][W][64];
+  const Where w(a, blockIdx.x);
+  const bool seq = a.y != nullptr;
+  auto out_in = [&](int t0) { return seq || (LSTM && t0 < w.end && w.end - t0 <= L); };
 
-  float carry = 0.f, prod = 1.f;
-  if constexpr (!AGG) {
-    const float* end = LEAKY ? a.d_h_last : a.d_c_last;
-    if (end) carry = end[w.state];
-    const f32x2* p = (const f32x2*)a.agg + w.state;
-    for (int s = a.segs - 1; s > seg; --s) {
-      const f32x2 e = p[(s - 1) * a.cols_all];
-      carry = __builtin_fmaf(e[0], carry, e[1]);
-    }
-  }
-
-  // chunks from the last to the first
-  int t = t_beg + (t_end - 1 - t_beg) / CH * CH;
-  const int last = t + w.wave * L;                      // this wave's first step in the last chunk
-  const int64_t x_at = w.base(a.xs, last), x_step = a.xs.t * CH;
+  float carry = a.h0 ? a.h0[w.state] : 0.f;
+  const int mine = w.wave * L;                          // this wave's first step
+  const int64_t x_at = w.base(a.xs, mine), x_step = a.xs.t * CH;
   const uint32_t xo = w.lane_off(a.xs, sizeof(T));
-  const int64_t d_at = AGG ? 0 : w.base(a.ds, last), d_step = a.ds.t * CH;
-  const uint32_t dof = AGG ? 0 : w.lane_off(a.ds, sizeof(T));
   const char* xp[G];
-  char* dp[G];
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    xp[g] = a.x[g] + x_at;
-    dp[g] = AGG ? nullptr : a.dx[g] + d_at;
-  }
-  const char* yp = has_dy ? a.y + w.base(a.ys, last) : nullptr;
-  const uint32_t yo = has_dy ? w.lane_off(a.ys, sizeof(T)) : 0;
+  for (int g = 0; g < G; ++g) xp[g] = a.x[g] + x_at;
+  char* yp = seq ? a.y + w.base(a.ys, mine) : nullptr;
+  const uint32_t yo = seq ? w.lane_off(a.ys, sizeof(T)) : 0;
 
-  T raw[G][L], rdy[L];
-  float nst = 0.f;                                      // the state before the fetched chunk
-  auto fetch = [&](int tc) {
-    const int t0 = tc + w.wave * L, live = lim - t0;
+  T raw[G][L];
+  auto fetch = [&](int t0) {
 #pragma unroll
-    for (int g = 0; g < (LEAKY ? AGG ? 1 : 2 : 3); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, live);
-    if constexpr (!LEAKY)
-      if (enters(t0)) load_steps(raw[3], xp[3], a.xs.t, xo, live);
+    for (int g = 0; g < (LSTM ? 3 : 2); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, w.end - t0);
+    if constexpr (LSTM) {                               // o is wanted for y, or at the row's last step
+      if (out_in(t0)) load_steps(raw[3], xp[3], a.xs.t, xo, w.end - t0);
       else forget(raw[3]);
-    if (has_dy) load_steps(rdy, yp, a.ys.t, yo, live);
-    if constexpr (!(AGG && LEAKY)) {
-      const float* s = tc > 0 ? a.saved + (tc / CH - 1) * a.cols_all : a.h0;
-      nst = s ? s[w.state] : 0.f;
     }
 #pragma unroll
-    for (int g = 0; g < G; ++g) xp[g] -= x_step;
-    if (has_dy) yp -= a.ys.t * CH;
+    for (int g = 0; g < G; ++g) xp[g] += x_step;
   };
-#pragma unroll
-  for (int l = 0; l < L; ++l) rdy[l] = (T)0.f;
+  fetch(mine);
 
-  for (; t >= t_beg && t >= lim; t -= CH) {             // behind the row's end dx is only cleared
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      xp[g] -= x_step;
-      if constexpr (!AGG) {
-        if (w.on) store_steps(rdy, dp[g], a.ds.t, dof, 0, t_end - (t + w.wave * L));
-        dp[g] -= d_step;
-      }
-    }
-    if (has_dy) yp -= a.ys.t * CH;
-  }
-  if (t >= t_beg) fetch(t);
   int par = 0;
-  for (; t >= t_beg; t -= CH) {
-    const int t0 = t + w.wave * L, live = lim - t0;
-    // a; what the gradients are made of; dy, then dL/dh_t through y_t
-    float A[L], K0[L], K1[L], D[L];
-    float B[L], K2[L], O[L], OP[L];                     // lstm
-    float cin = nst;
+  for (int t = 0; t < a.T; t += CH) {
+    const int t0 = t + mine, live = w.end - t0, room = a.T - t0;
+    if (t >= w.end) {                                   // the whole chunk is behind the row's end
+      if (!seq) break;
+      if (w.on) store_steps(raw[0], yp, a.ys.t, yo, 0, room);
+      yp += a.ys.t * CH;
+      continue;
+    }
+    Fwd<FORM, T, L> f;
+    f.make(raw, out_in(t0));
+    if (t + CH < w.end) {
+      fetch(t0 + CH);
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) forget(raw[g]);
+    }
+    f.end_row(live);
+
+    float cin = carry;
+    if constexpr (W > 1) {
+      pq[par][w.wave][w.lane] = f.piece();
+      lds_barrier();
+      // compose: the state before this wave's steps, and the one after the chunk
+      const int wave = here(w.wave);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const f32x2 e = pq[par][k][w.lane];
+        cin = k == wave ? carry : cin;
+        carry = __builtin_fmaf(e[0], carry, e[1]);
+      }
+      par ^= 1;
+      // where the backward's chunks begin
+      if (a.saved && (w.wave == 0 || w.wave == W / 2) && t0 > 0 && t0 < a.T && w.on)
+        a.saved[(t0 / (CH / 2) - 1) * a.cols_all + w.state] = cin;
+    }
+    const float after = f.finish(a, w, cin, t0, live, room, seq, out_in(t0), yp, yo);
+    if constexpr (W == 1) carry = after;
+    if (seq) yp += a.ys.t * CH;
+  }
+  if (w.wave == 0) last_states<FORM>(a, w, carry);
+}
+
+// ------------------------------------------------------------------ a wave's steps, backward
+
+template <int FORM, typename T, int L> struct Bwd {
+  static constexpr int G = gates_of<FORM>();
+  static constexpr bool LEAKY = FORM == PT_SCAN_LEAKY, ACC = sizeof(T) == 4;
+  // a; what the gradients are made of; dy, then dL/dh_t through y_t
+  float A[L], K0[L], K1[L], D[L];
+  float B[L], K2[L], O[L], OP[L];                       // lstm
+
+  __device__ __forceinline__ void make(const T (&raw)[G][L], const T (&rdy)[L], bool enters) {
 #pragma unroll
     for (int l = 0; l < L; ++l) {
       D[l] = (float)rdy[l];
       if constexpr (LEAKY) {
         const Logistic z = logistic<ACC>(as_f32(raw[0][l]));
         A[l] = z.sm;
-        if constexpr (!AGG) {
-          K1[l] = z.s;
-          K0[l] = as_f32(raw[1][l]);
-        }
+        K1[l] = z.s;
+        K0[l] = as_f32(raw[1][l]);
       } else {
         const Logistic f = logistic<ACC>(as_f32(raw[1][l])), i = logistic<ACC>(as_f32(raw[0][l]));
         float d;
@@ -534,7 +468,7 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
       }
     }
     if constexpr (!LEAKY) {
-      if (enters(t0)) {
+      if (enters) {
 #pragma unroll
         for (int l = 0; l < L; ++l) {
           const Logistic g = logistic<ACC>(as_f32(raw[3][l]));
@@ -545,77 +479,52 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
         forget(O);
         forget(OP);
       }
-    }
-    settle(A);
-    settle(D);
-    if constexpr (!(LEAKY && AGG)) {
-      settle(K0);
-      settle(K1);
-    }
-    if constexpr (!LEAKY) {
       settle(B);
       settle(K2);
     }
-    if (t > t_beg) {
-      fetch(t - CH);
-    } else {
+    settle(A);
+    settle(D);
+    settle(K0);
+    settle(K1);
+  }
+  __device__ __forceinline__ void end_row(int live) {   // behind the row's end: h' = h, dx = 0
+    if (live >= L) return;
 #pragma unroll
-      for (int g = 0; g < G; ++g) forget(raw[g]);
-      if (has_dy) forget(rdy);
-    }
-    if (live < L) {                                     // behind the row's end: h' = h, dx = 0
-#pragma unroll
-      for (int l = 0; l < L; ++l)
-        if (l >= live) {
-          A[l] = 1.f;
-          if constexpr (!LEAKY) B[l] = 0.f;
-          else if constexpr (!AGG) K1[l] = 0.f;
-        }
-      settle(A);
-      if constexpr (!LEAKY) settle(B);
-      else if constexpr (!AGG) settle(K1);
-    }
-
-    float gin = carry;
-    if constexpr (W > 1) {
-      f32x2 own = {A[0], 0.f};
-#pragma unroll
-      for (int l = 1; l < L; ++l) own[0] *= A[l];
-      if constexpr (!LEAKY || !AGG) {
-#pragma unroll
-        for (int l = 0; l < L; ++l) own[1] = __builtin_fmaf(A[l], own[1], LEAKY ? K1[l] * K0[l] : B[l]);
+    for (int l = 0; l < L; ++l)
+      if (l >= live) {
+        A[l] = 1.f;
+        if constexpr (LEAKY) K1[l] = 0.f; else B[l] = 0.f;
       }
-      pq[par][w.wave][w.lane] = own;
-      if constexpr (LEAKY) {                            // y = h: dy needs no state
-        float g = 0.f;
+    settle(A);
+    if constexpr (LEAKY) settle(K1); else settle(B);
+  }
+  __device__ __forceinline__ f32x2 piece() const {
+    f32x2 e = {A[0], LEAKY ? K1[0] * K0[0] : B[0]};
 #pragma unroll
-        for (int l = L - 1; l >= 0; --l) g = A[l] * (D[l] + g);
-        gq[par][w.wave][w.lane] = g;
-      }
-      lds_barrier();
-      if constexpr (!(AGG && LEAKY)) {
-        const int wave = here(w.wave);
+    for (int l = 1; l < L; ++l)
+      e = f32x2{e[0] * A[l], __builtin_fmaf(A[l], e[1], LEAKY ? K1[l] * K0[l] : B[l])};
+    return e;
+  }
+  // What leaves the steps towards the past when nothing comes from behind.
+  __device__ __forceinline__ float gradient_out() const {
+    float g = 0.f;
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-          const f32x2 e = pq[par][k][w.lane];
-          cin = k < wave ? __builtin_fmaf(e[0], cin, e[1]) : cin;
-        }
-      }
-    }
-
-    // the states, forward
+    for (int l = L - 1; l >= 0; --l) g = A[l] * (D[l] + g);
+    return g;
+  }
+  // The states, from c on; the o gate's gradient is written.
+  __device__ __forceinline__ void walk(const Args& a, const Where& w, float c, int t0, int live, int room, bool enters,
+                                       char* dp3, uint32_t dof) {
     if constexpr (LEAKY) {
-      if constexpr (!AGG) {
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
-          const float n = K0[l], s = K1[l];
-          K0[l] = (n - cin) * (s * A[l]);
-          cin = __builtin_fmaf(A[l], cin, s * n);
-        }
+      for (int l = 0; l < L; ++l) {
+        const float n = K0[l], s = K1[l];
+        K0[l] = (n - c) * (s * A[l]);
+        c = __builtin_fmaf(A[l], c, s * n);
       }
     } else {
       T out[L];
-      if (enters(t0)) {
+      if (enters) {
         if (a.d_h_last && t0 < w.end && w.end - t0 <= L) {
           const float e = a.d_h_last[w.state];
 #pragma unroll
@@ -624,68 +533,380 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
         }
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-          K1[l] *= cin;
-          cin = __builtin_fmaf(A[l], cin, B[l]);
+          K1[l] *= c;
+          c = __builtin_fmaf(A[l], c, B[l]);
           float d;
-          const float th = tanh_d<ACC>(cin, d);
+          const float th = tanh_d<ACC>(c, d);
           out[l] = (T)(D[l] * th * OP[l]);
           D[l] *= O[l] * d;
         }
       } else {
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-          K1[l] *= cin;
-          cin = __builtin_fmaf(A[l], cin, B[l]);
+          K1[l] *= c;
+          c = __builtin_fmaf(A[l], c, B[l]);
           out[l] = (T)0.f;
         }
       }
-      if constexpr (!AGG) {
-        if (w.on) store_steps(out, dp[3], a.ds.t, dof, live, t_end - t0);
-        dp[3] -= d_step;
-      }
-      if constexpr (W > 1) {
-        float g = 0.f;
-#pragma unroll
-        for (int l = L - 1; l >= 0; --l) g = A[l] * (D[l] + g);
-        gq[par][w.wave][w.lane] = g;
-        lds_barrier();
-      }
+      if (w.on) store_steps(out, dp3, a.ds.t, dof, live, room);
     }
-    if constexpr (W > 1) {
-      const int wave = here(w.wave);
-#pragma unroll
-      for (int k = W - 1; k >= 0; --k) {
-        const float p = pq[par][k][w.lane][0];
-        gin = k == wave ? carry : gin;
-        carry = __builtin_fmaf(p, carry, gq[par][k][w.lane]);
-        if constexpr (AGG) prod *= p;
-      }
-      par ^= 1;
-    }
-    if constexpr (AGG) continue;
-
+  }
+  // The other gates' gradients, with g coming from behind; returns what leaves.
+  __device__ __forceinline__ float finish(const Args& a, const Where& w, float g, int live, int room,
+                                          char* const (&dp)[G], uint32_t dof) {
     T out[3][L];
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
-      const float g = D[l] + gin;
-      out[0][l] = (T)(g * K0[l]);
-      out[1][l] = (T)(g * K1[l]);
-      if constexpr (!LEAKY) out[2][l] = (T)(g * K2[l]);
-      gin = A[l] * g;
+      const float t = D[l] + g;
+      out[0][l] = (T)(t * K0[l]);
+      out[1][l] = (T)(t * K1[l]);
+      if constexpr (!LEAKY) out[2][l] = (T)(t * K2[l]);
+      g = A[l] * t;
     }
 #pragma unroll
-    for (int g = 0; g < (LEAKY ? 2 : 3); ++g) {
-      if (w.on) store_steps(out[g], dp[g], a.ds.t, dof, live, t_end - t0);
+    for (int k = 0; k < (LEAKY ? 2 : 3); ++k)
+      if (w.on) store_steps(out[k], dp[k], a.ds.t, dof, live, room);
+    return g;
+  }
+};
+
+// lstm: whether any gradient enters through y among the L steps from t0 (without
+// a dy it does at the row's last step alone, and o, tanh(c) matter only there).
+__device__ __forceinline__ bool enters_in(const Args& a, const Where& w, int t0, int L) {
+  return a.y != nullptr || (a.d_h_last && t0 < w.end && w.end - t0 <= L);
+}
+
+// The gradient of the state after a row's last step.
+template <int FORM> __device__ __forceinline__ float end_gradient(const Args& a, const Where& w) {
+  const float* end = FORM == PT_SCAN_LEAKY ? a.d_h_last : a.d_c_last;
+  return end ? end[w.state] : 0.f;
+}
+
+// Backward, a workgroup walking a column tile's whole row from its end.
+template <int FORM, typename T, int W>
+__global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
+  constexpr int G = gates_of<FORM>(), L = back_steps<FORM>(), CH = W * L;
+  constexpr bool LEAKY = FORM == PT_SCAN_LEAKY;
+  __shared__ f32x2 pq[2][W][64];              // forward (P, q); two sets in turn, as in the forward
+  __shared__ float gq[2][W][64];              // backward q (its P is the same)
+  const Where w(a, blockIdx.x);
+  const bool has_dy = a.y != nullptr;
+  float carry = end_gradient<FORM>(a, w);
+
+  // chunks from the last to the first
+  int t = (a.T - 1) / CH * CH;
+  const int last = t + w.wave * L;                      // this wave's first step in the last chunk
+  const int64_t x_at = w.base(a.xs, last), x_step = a.xs.t * CH;
+  const uint32_t xo = w.lane_off(a.xs, sizeof(T));
+  const int64_t d_at = w.base(a.ds, last), d_step = a.ds.t * CH;
+  const uint32_t dof = w.lane_off(a.ds, sizeof(T));
+  const char* xp[G];
+  char* dp[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    xp[g] = a.x[g] + x_at;
+    dp[g] = a.dx[g] + d_at;
+  }
+  const char* yp = has_dy ? a.y + w.base(a.ys, last) : nullptr;
+  const uint32_t yo = has_dy ? w.lane_off(a.ys, sizeof(T)) : 0;
+
+  T raw[G][L], rdy[L];
+  float nst = 0.f;                                      // the state before the fetched chunk
+  auto fetch = [&](int tc) {
+    const int t0 = tc + w.wave * L, live = w.end - t0;
+#pragma unroll
+    for (int g = 0; g < (LEAKY ? 2 : 3); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, live);
+    if constexpr (!LEAKY) {
+      if (enters_in(a, w, t0, L)) load_steps(raw[3], xp[3], a.xs.t, xo, live);
+      else forget(raw[3]);
+    }
+    if (has_dy) load_steps(rdy, yp, a.ys.t, yo, live);
+    const float* s = tc > 0 ? a.saved + (tc / CH - 1) * a.cols_all : a.h0;
+    nst = s ? s[w.state] : 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) xp[g] -= x_step;
+    if (has_dy) yp -= a.ys.t * CH;
+  };
+#pragma unroll
+  for (int l = 0; l < L; ++l) rdy[l] = (T)0.f;
+
+  for (; t >= 0 && t >= w.end; t -= CH) {               // behind the row's end dx is only cleared
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      xp[g] -= x_step;
+      if (w.on) store_steps(rdy, dp[g], a.ds.t, dof, 0, a.T - (t + w.wave * L));
       dp[g] -= d_step;
     }
-    if constexpr (W == 1) carry = gin;
+    if (has_dy) yp -= a.ys.t * CH;
   }
+  if (t >= 0) fetch(t);
+  int par = 0;
+  for (; t >= 0; t -= CH) {
+    const int t0 = t + w.wave * L, live = w.end - t0, room = a.T - t0;
+    const bool enters = enters_in(a, w, t0, L);
+    float cin = nst;
+    Bwd<FORM, T, L> b;
+    b.make(raw, rdy, enters);
+    if (t > 0) {
+      fetch(t - CH);
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) forget(raw[g]);
+      if (has_dy) forget(rdy);
+    }
+    b.end_row(live);
 
-  if (w.wave != 0 || !w.on) return;
-  if constexpr (AGG)
-    ((f32x2*)a.agg)[w.seg * a.cols_all + w.state] = f32x2{prod, carry};
-  else if (seg == 0 && a.d_h0)
-    a.d_h0[w.state] = carry;
+    float gin = carry;
+    if constexpr (W > 1) {
+      pq[par][w.wave][w.lane] = b.piece();
+      if constexpr (LEAKY) gq[par][w.wave][w.lane] = b.gradient_out();      // y = h: dy needs no state
+      lds_barrier();
+      const int wave = here(w.wave);
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k) {
+        const f32x2 e = pq[par][k][w.lane];
+        cin = k < wave ? __builtin_fmaf(e[0], cin, e[1]) : cin;
+      }
+    }
+    b.walk(a, w, cin, t0, live, room, enters, dp[G - 1], dof);
+    if constexpr (W > 1) {
+      if constexpr (!LEAKY) {
+        gq[par][w.wave][w.lane] = b.gradient_out();
+        lds_barrier();
+      }
+      const int wave = here(w.wave);
+#pragma unroll
+      for (int k = W - 1; k >= 0; --k) {
+        gin = k == wave ? carry : gin;
+        carry = __builtin_fmaf(pq[par][k][w.lane][0], carry, gq[par][k][w.lane]);
+      }
+      par ^= 1;
+    }
+    const float out = b.finish(a, w, gin, live, room, dp, dof);
+    if constexpr (W == 1) carry = out;
+#pragma unroll
+    for (int g = 0; g < G; ++g) dp[g] -= d_step;
+  }
+  if (w.wave == 0 && w.on && a.d_h0) a.d_h0[w.state] = carry;
+}
+
+// ------------------------------------------------------------------ the chain
+//
+// Workgroups take numbers from a ticket, so whatever a workgroup waits for was
+// taken up before it and waits itself only for still earlier ones: every wait
+// ends, whatever order the card starts them in.  A pair is one 64-bit word that
+// is written once, so a reader sees none of it or all of it, and needs no fence:
+// nothing but the word is handed over.  NOT_YET is what no pair can be (its P
+// would be a NaN of a form that is never published).
+
+constexpr uint64_t NOT_YET = ~(uint64_t)0;
+constexpr int CHAIN_HEAD = 256;          // bytes of the ticket, in front of the pairs
+
+// The ticket to 0 and every pair to NOT_YET, `n` times 16 bytes.
+__global__ __launch_bounds__(256) void k_chain_clear(vec<uint32_t, 4>* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    p[i] = i < CHAIN_HEAD / 16 ? (vec<uint32_t, 4>)(0u) : (vec<uint32_t, 4>)(~0u);
+}
+
+__device__ __forceinline__ uint32_t chain_number(uint32_t* ticket) {
+  __shared__ uint32_t id;
+  if (threadIdx.x == 0) id = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(id);
+}
+
+__device__ __forceinline__ void publish(uint64_t* slot, float p, float q) {
+  const uint32_t pb = p != p ? 0x7fc00000u : __builtin_bit_cast(uint32_t, p);
+  __hip_atomic_store(slot, (uint64_t)__builtin_bit_cast(uint32_t, q) << 32 | pb, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* slot) {
+  return __hip_atomic_load(slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The pair, from a first look at it.  (Idle lanes look at column 0's, which is published as well.)
+__device__ __forceinline__ f32x2 await(const uint64_t* slot, uint64_t v) {
+  while (__any(v == NOT_YET)) {
+    __builtin_amdgcn_s_sleep(1);
+    v = peek(slot);
+  }
+  return f32x2{__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32))};
+}
+
+// One wave's part of the pairs of `count` chunks from `slot` on, `step` words apart,
+// joined in this order: the waves look at them side by side, one round trip to
+// memory for all.
+template <int W>
+__device__ __forceinline__ f32x2 join(const uint64_t* slot, int64_t step, int count, int wave) {
+  constexpr int N = GROUP / W;
+  count -= wave * N;
+  slot += wave * N * step;
+  uint64_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = i < count ? peek(slot + i * step) : 0;
+  f32x2 e = {1.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < count) {
+      const f32x2 n = await(slot + i * step, v[i]);
+      e = f32x2{e[0] * n[0], __builtin_fmaf(n[0], e[1], n[1])};
+    }
+  return e;
+}
+
+template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) void k_chain_fwd(Args a) {
+  constexpr int W = CHAIN_FWD, G = gates_of<FORM>(), L = chain_steps<FORM>(), CH = W * L;
+  constexpr bool LSTM = FORM == PT_SCAN_LSTM;
+  __shared__ f32x2 pq[W][64], pj[W][64];  // the waves' pieces; their parts of the join
+  __shared__ float cs[64];               // what the join starts from
+  const Where w(a, chain_number(a.ticket));
+  const int t_beg = w.seg * CH, t0 = t_beg + w.wave * L, live = w.end - t0, room = a.T - t0;
+  const bool seq = a.y != nullptr;
+  char* yp = seq ? a.y + w.base(a.ys, t0) : nullptr;
+  const uint32_t yo = seq ? w.lane_off(a.ys, sizeof(T)) : 0;
+  if (t_beg >= w.end) {                  // behind the row's end: nobody waits for this chunk
+    const T none[L] = {};
+    if (seq && w.on) store_steps(none, yp, a.ys.t, yo, 0, room);
+    if (w.seg == 0 && w.wave == 0) last_states<FORM>(a, w, a.h0 ? a.h0[w.state] : 0.f);
+    return;
+  }
+  const bool out_here = seq || (LSTM && t0 < w.end && w.end - t0 <= L);
+  const int64_t x_at = w.base(a.xs, t0);
+  const uint32_t xo = w.lane_off(a.xs, sizeof(T));
+  T raw[G][L];
+#pragma unroll
+  for (int g = 0; g < (LSTM ? 3 : 2); ++g) load_steps(raw[g], a.x[g] + x_at, a.xs.t, xo, live);
+  if constexpr (LSTM) {
+    if (out_here) load_steps(raw[3], a.x[3] + x_at, a.xs.t, xo, live);
+    else forget(raw[3]);
+  }
+  Fwd<FORM, T, L> f;
+  f.make(raw, out_here);
+  f.end_row(live);
+  pq[w.wave][w.lane] = f.piece();
+  lds_barrier();
+  const int first = w.seg & -GROUP, group = w.seg / GROUP;
+  const bool more = t_beg + CH < w.end;                 // a later chunk waits for this one
+  f32x2 own = {1.f, 0.f};                               // wave 0: the chunk's pair
+  if (w.wave == 0) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const f32x2 n = pq[k][w.lane];
+      own = f32x2{own[0] * n[0], __builtin_fmaf(n[0], own[1], n[1])};
+    }
+    if (more && w.on) publish(a.pairs + w.seg * a.cols_all + w.state, own[0], own[1]);
+    if (first == 0) {
+      cs[w.lane] = a.h0 ? a.h0[w.state] : 0.f;
+    } else {
+      const uint64_t* s = a.states + (group - 1) * a.cols_all + w.state;
+      cs[w.lane] = await(s, peek(s))[1];
+    }
+  }
+  pj[w.wave][w.lane] = join<W>(a.pairs + first * a.cols_all + w.state, a.cols_all, w.seg - first, w.wave);
+  lds_barrier();
+  float c = cs[w.lane];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    const f32x2 e = pj[k][w.lane];
+    c = __builtin_fmaf(e[0], c, e[1]);
+  }
+  if (w.wave == 0) {
+    const float after = __builtin_fmaf(own[0], c, own[1]);
+    if (more && (w.seg + 1) % GROUP == 0 && w.on) publish(a.states + group * a.cols_all + w.state, 1.f, after);
+    if (!more) last_states<FORM>(a, w, after);
+  }
+  for (int k = 0; k < w.wave; ++k) {
+    const f32x2 e = pq[k][w.lane];
+    c = __builtin_fmaf(e[0], c, e[1]);
+  }
+  // where the backward's chunks begin
+  if (a.saved && (w.wave == 0 || w.wave == W / 2) && t0 > 0 && t0 < a.T && w.on)
+    a.saved[(t0 / (CH / 2) - 1) * a.cols_all + w.state] = c;
+  f.finish(a, w, c, t0, live, room, seq, out_here, yp, yo);
+}
+
+template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_BWD, 4) void k_chain_bwd(Args a) {
+  constexpr int W = CHAIN_BWD, G = gates_of<FORM>(), L = chain_steps<FORM>(), CH = W * L;
+  constexpr bool LEAKY = FORM == PT_SCAN_LEAKY;
+  __shared__ f32x2 pq[W][64], pj[W][64];  // as in the forward; gq: the pieces' q backward
+  __shared__ float gq[W][64], cs[64];
+  Where w(a, chain_number(a.ticket));
+  w.seg = a.segs - 1 - w.seg;            // from the far end
+  const int t_beg = w.seg * CH, t0 = t_beg + w.wave * L, live = w.end - t0, room = a.T - t0;
+  const bool has_dy = a.y != nullptr;
+  const int64_t d_at = w.base(a.ds, t0);
+  const uint32_t dof = w.lane_off(a.ds, sizeof(T));
+  char* dp[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) dp[g] = a.dx[g] + d_at;
+  if (t_beg >= w.end) {                  // behind the row's end: nobody waits for this chunk
+    const T none[L] = {};
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (w.on) store_steps(none, dp[g], a.ds.t, dof, 0, room);
+    if (w.seg == 0 && w.wave == 0 && w.on && a.d_h0) a.d_h0[w.state] = end_gradient<FORM>(a, w);
+    return;
+  }
+  const bool enters = enters_in(a, w, t0, L);
+  const int64_t x_at = w.base(a.xs, t0);
+  const uint32_t xo = w.lane_off(a.xs, sizeof(T));
+  T raw[G][L], rdy[L] = {};
+#pragma unroll
+  for (int g = 0; g < (LEAKY ? 2 : 3); ++g) load_steps(raw[g], a.x[g] + x_at, a.xs.t, xo, live);
+  if constexpr (!LEAKY) {
+    if (enters) load_steps(raw[3], a.x[3] + x_at, a.xs.t, xo, live);
+    else forget(raw[3]);
+  }
+  if (has_dy) load_steps(rdy, a.y + w.base(a.ys, t0), a.ys.t, w.lane_off(a.ys, sizeof(T)), live);
+  const float* s = w.seg > 0 ? a.saved + (w.seg - 1) * a.cols_all : a.h0;
+  float cin = s ? s[w.state] : 0.f;
+  Bwd<FORM, T, L> b;
+  b.make(raw, rdy, enters);
+  b.end_row(live);
+  pq[w.wave][w.lane] = b.piece();
+  if constexpr (LEAKY) gq[w.wave][w.lane] = b.gradient_out();
+  lds_barrier();
+  for (int k = 0; k < w.wave; ++k) {
+    const f32x2 e = pq[k][w.lane];
+    cin = __builtin_fmaf(e[0], cin, e[1]);
+  }
+  b.walk(a, w, cin, t0, live, room, enters, dp[G - 1], dof);
+  if constexpr (!LEAKY) {
+    gq[w.wave][w.lane] = b.gradient_out();
+    lds_barrier();
+  }
+  const int far = (w.end - 1) / CH;                     // the row's last chunk
+  const int group = w.seg / GROUP, next = (group + 1) * GROUP;
+  const int from = next > far ? far : next - 1;         // the last chunk whose pair is joined
+  f32x2 own = {1.f, 0.f};                               // wave 0: the chunk's pair
+  if (w.wave == 0) {
+#pragma unroll
+    for (int k = W - 1; k >= 0; --k) {
+      const float p = pq[k][w.lane][0];
+      own = f32x2{own[0] * p, __builtin_fmaf(p, own[1], gq[k][w.lane])};
+    }
+    if (w.seg > 0 && w.on) publish(a.pairs + w.seg * a.cols_all + w.state, own[0], own[1]);
+    if (next > far) {
+      cs[w.lane] = end_gradient<FORM>(a, w);
+    } else {
+      const uint64_t* st = a.states + (group + 1) * a.cols_all + w.state;
+      cs[w.lane] = await(st, peek(st))[1];
+    }
+  }
+  pj[w.wave][w.lane] = join<W>(a.pairs + from * a.cols_all + w.state, -a.cols_all, from - w.seg, w.wave);
+  lds_barrier();
+  float g = cs[w.lane];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    const f32x2 e = pj[k][w.lane];
+    g = __builtin_fmaf(e[0], g, e[1]);
+  }
+  if (w.wave == 0) {
+    const float out = __builtin_fmaf(own[0], g, own[1]);
+    if (w.seg > 0 && w.seg % GROUP == 0 && w.on) publish(a.states + group * a.cols_all + w.state, 1.f, out);
+    if (w.seg == 0 && w.on && a.d_h0) a.d_h0[w.state] = out;
+  }
+  for (int k = W - 1; k > w.wave; --k) g = __builtin_fmaf(pq[k][w.lane][0], g, gq[k][w.lane]);
+  b.finish(a, w, g, live, room, dp, dof);
 }
 
 // One step: element-wise, one lane per V columns.
@@ -744,40 +965,43 @@ int check(const pt_scan_desc* d) {
 // How a shape is cut; from the descriptor alone, so that forward, backward and
 // the size queries agree.
 struct Plan {
-  int W;
+  int W;                     // 0: the chain
   int64_t chunk, nchunks;    // of the backward; the forward's are two of them
-  int segs, seg_steps;
 };
 
-// The waves that share a column tile, and the pieces that time is cut into, by
-// the column tiles there are.  The card holds 256 workgroups of 16 waves at a
-// time, or 512 of 8 (registers), or 1024 and more of 4:
+// The waves that share a column tile, by the column tiles there are.  The card
+// holds 256 workgroups of 16 waves at a time, or 512 of 8 (registers), or 1024
+// and more of 4:
 //   tiles > 512   4 waves.  More waves only make each chunk's exchange longer
 //                 (2048 tiles of 300 steps, leaky bf16: forward 48 us, 58 with 8;
 //                 700 of 4096: 262, 269).
 //   257 .. 512    8 waves (300 tiles of 4096 steps: 146 us, 162 with 4 or 16).
 //   129 .. 256    16 waves: one workgroup a compute unit (180 tiles: 81 us, 136
-//                 with 4, 108 with 8 in two pieces).
-//   up to 128     8 waves and 512 / tiles pieces of time, at the price of reading
-//                 the gates twice (64 tiles of 4096: 43 us, 118 unsplit, 46 with 16
-//                 waves in 4 pieces; 110 tiles: 67, and 71 in 16 waves and 2 pieces).
+//                 with 4, 108 with 8).
+//   up to 128     the chain, from more than one of its forward's chunks on; else 8
+//                 waves.
 // Up to 4 L steps fit a chunk of 4 waves, up to L steps one wave.
 Plan plan_of(const pt_scan_desc* d) {
   Plan p;
-  const int L = d->form == PT_SCAN_LEAKY ? back_steps<PT_SCAN_LEAKY>() : back_steps<PT_SCAN_LSTM>();
+  const bool leaky = d->form == PT_SCAN_LEAKY;
+  const int L = leaky ? back_steps<PT_SCAN_LEAKY>() : back_steps<PT_SCAN_LSTM>();
+  const int chain = CHAIN_BWD * (leaky ? chain_steps<PT_SCAN_LEAKY>() : chain_steps<PT_SCAN_LSTM>());
   const int64_t tiles = d->batch * ((d->channels * d->inner + 63) / 64);
   if (d->steps <= L) p.W = 1;
   else if (d->steps <= 4 * L || tiles > 512) p.W = 4;
-  else p.W = tiles > 128 && tiles <= 256 ? 16 : SPLIT_W;
-  p.chunk = (int64_t)p.W * L;
+  else if (tiles > 256) p.W = 8;
+  else if (tiles > 128) p.W = 16;
+  else p.W = d->steps > 2 * chain ? 0 : 8;
+  p.chunk = p.W ? (int64_t)p.W * L : chain;
   p.nchunks = (d->steps + p.chunk - 1) / p.chunk;
-  const int64_t pairs = (p.nchunks + 1) / 2;
-  int64_t segs = 1;
-  if (p.W == SPLIT_W && tiles <= 128) segs = std::min<int64_t>(std::min<int64_t>(512 / tiles, pairs), MAX_SEGS);
-  const int64_t per = (pairs + segs - 1) / segs;
-  p.segs = (int)((pairs + per - 1) / per);
-  p.seg_steps = (int)std::min<int64_t>(per * 2 * p.chunk, (int64_t)1 << 30);
   return p;
+}
+
+// The chain's scratch: the ticket, a pair per chunk (of the backward: the most),
+// a state per group of chunks.
+size_t chain_bytes(const pt_scan_desc* d, const Plan& p) {
+  const int64_t words = (p.nchunks + (p.nchunks + GROUP - 1) / GROUP) * d->batch * d->channels * d->inner;
+  return p.W ? 0 : CHAIN_HEAD + ((size_t)words * sizeof(uint64_t) + 15) / 16 * 16;
 }
 
 // Strides of axes of one element never count: 0, so that they cannot spoil the alignment.
@@ -797,36 +1021,26 @@ bool spans32(const pt_scan_desc* d, const pt_scan_view& v, int size) {
   return v.sc >= 0 && s < 2147483648.0;
 }
 
-template <int FORM, typename T, int W>
-int launch_fwd(Args a, int64_t blocks, hipStream_t s) {
-  if constexpr (W == SPLIT_W)
-    if (a.segs > 1) {
-      const int64_t n = blocks / a.segs * (a.segs - 1);
-      hipLaunchKernelGGL((k_scan_fwd<FORM, T, W, true>), dim3((unsigned)n), dim3(64 * W), 0, s, a);
-    }
-  hipLaunchKernelGGL((k_scan_fwd<FORM, T, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
-  return hipGetLastError() == hipSuccess ? 0 : fail(PT_SCAN_ERR_HIP, "scan: forward launch failed");
+template <int FORM, typename T, int W> void launch_rows(const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
+  if (bwd) hipLaunchKernelGGL((k_scan_bwd<FORM, T, W>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
+  else hipLaunchKernelGGL((k_scan_fwd<FORM, T, W>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
 }
 
-template <int FORM, typename T, int W>
-int launch_bwd(Args a, int64_t blocks, hipStream_t s) {
-  if constexpr (W == SPLIT_W)
-    if (a.segs > 1) {
-      const int64_t n = blocks / a.segs * (a.segs - 1);
-      hipLaunchKernelGGL((k_scan_bwd<FORM, T, W, true>), dim3((unsigned)n), dim3(64 * W), 0, s, a);
-    }
-  hipLaunchKernelGGL((k_scan_bwd<FORM, T, W, false>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
-  return hipGetLastError() == hipSuccess ? 0 : fail(PT_SCAN_ERR_HIP, "scan: backward launch failed");
+template <int FORM, typename T> void launch_chain(const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
+  if (bwd) hipLaunchKernelGGL((k_chain_bwd<FORM, T>), dim3((unsigned)blocks), dim3(64 * CHAIN_BWD), 0, s, a);
+  else hipLaunchKernelGGL((k_chain_fwd<FORM, T>), dim3((unsigned)blocks), dim3(64 * CHAIN_FWD), 0, s, a);
 }
 
 template <int FORM, typename T>
 int launch_w(const Plan& p, const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
   switch (p.W) {
-    case 1: return bwd ? launch_bwd<FORM, T, 1>(a, blocks, s) : launch_fwd<FORM, T, 1>(a, blocks, s);
-    case 16: return bwd ? launch_bwd<FORM, T, 16>(a, blocks, s) : launch_fwd<FORM, T, 16>(a, blocks, s);
-    case 4: return bwd ? launch_bwd<FORM, T, 4>(a, blocks, s) : launch_fwd<FORM, T, 4>(a, blocks, s);
-    default: return bwd ? launch_bwd<FORM, T, SPLIT_W>(a, blocks, s) : launch_fwd<FORM, T, SPLIT_W>(a, blocks, s);
+    case 0: launch_chain<FORM, T>(a, blocks, bwd, s); break;
+    case 1: launch_rows<FORM, T, 1>(a, blocks, bwd, s); break;
+    case 4: launch_rows<FORM, T, 4>(a, blocks, bwd, s); break;
+    case 8: launch_rows<FORM, T, 8>(a, blocks, bwd, s); break;
+    default: launch_rows<FORM, T, 16>(a, blocks, bwd, s);
   }
+  return hipGetLastError() == hipSuccess ? 0 : fail(PT_SCAN_ERR_HIP, "scan: launch failed");
 }
 
 template <int FORM>
@@ -866,7 +1080,7 @@ struct Tensors {
   }
 };
 
-int run(const pt_scan_desc* d, const Plan& p, const Tensors& ts, Args& a, bool bwd, hipStream_t s) {
+int run(const pt_scan_desc* d, const Plan& p, const Tensors& ts, Args& a, void* workspace, bool bwd, hipStream_t s) {
   // Columns of one channel at a time where the inner axis fills whole tiles, or
   // where the channels of a step reach over more than a 32-bit offset.
   const bool grouped = ts.grouped && d->inner % 64 != 0 &&
@@ -878,13 +1092,22 @@ int run(const pt_scan_desc* d, const Plan& p, const Tensors& ts, Args& a, bool b
   a.cg = grouped ? d->channels : 1;
   a.groups = d->channels / a.cg;
   a.outer = d->batch * a.groups;
-  a.segs = p.segs;
-  a.seg_steps = p.seg_steps;
+  a.segs = p.W ? 1 : (int)(bwd ? p.nchunks : (p.nchunks + 1) / 2);
   const int64_t tiles = (a.cg * a.N + 63) / 64;
   a.tiles = (int)tiles;
-  if ((double)tiles * (double)a.outer * (double)p.segs > 2147483647.0)
+  if ((double)tiles * (double)a.outer * (double)a.segs > 2147483647.0)
     return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: too many columns for one launch");
-  const int64_t blocks = tiles * a.outer * p.segs;
+  if (!p.W) {
+    if (!workspace || (uintptr_t)workspace % 16)
+      return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace, aligned to 16 bytes");
+    a.ticket = (uint32_t*)workspace;
+    a.pairs = (uint64_t*)((char*)workspace + CHAIN_HEAD);
+    a.states = a.pairs + p.nchunks * a.cols_all;
+    const int64_t n = (int64_t)(chain_bytes(d, p) / 16);
+    hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, s,
+                       (vec<uint32_t, 4>*)workspace, n);
+  }
+  const int64_t blocks = tiles * a.outer * a.segs;
   return d->form == PT_SCAN_LEAKY ? launch_t<PT_SCAN_LEAKY>(d->dtype, p, a, blocks, bwd, s)
                                   : launch_t<PT_SCAN_LSTM>(d->dtype, p, a, blocks, bwd, s);
 }
@@ -904,8 +1127,7 @@ size_t pt_scan_saved_bytes(const pt_scan_desc* d) {
 
 size_t pt_scan_workspace_bytes(const pt_scan_desc* d) {
   if (check(d)) return 0;
-  const Plan p = plan_of(d);
-  return (size_t)((p.segs - 1) * d->batch * d->channels * d->inner) * 2 * sizeof(float);
+  return chain_bytes(d, plan_of(d));
 }
 
 int pt_scan_forward(const pt_scan_desc* d, const pt_scan_view* x, const float* h0, const int64_t* lengths,
@@ -919,11 +1141,9 @@ int pt_scan_forward(const pt_scan_desc* d, const pt_scan_view* x, const float* h
   ts.take(x, gates(d->form), a.x, a.xs, ts.size);
   if (y && y->data) ts.take(y, 1, &a.y, a.ys, ts.size);
   if (ts.rc) return ts.rc;
-  if (p.segs > 1 && !workspace) return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace");
   a.h0 = h0; a.len = lengths; a.h_last = h_last; a.c_last = c_last;
   a.saved = p.nchunks > 1 ? (float*)saved : nullptr;
-  a.agg = (float*)workspace;
-  return run(d, p, ts, a, false, (hipStream_t)stream);
+  return run(d, p, ts, a, workspace, false, (hipStream_t)stream);
 }
 
 int pt_scan_backward(const pt_scan_desc* d, const pt_scan_view* x, const float* h0, const int64_t* lengths,
@@ -939,11 +1159,9 @@ int pt_scan_backward(const pt_scan_desc* d, const pt_scan_view* x, const float* 
   if (dy && dy->data) ts.take(dy, 1, &a.y, a.ys, ts.size);
   if (ts.rc) return ts.rc;
   if (p.nchunks > 1 && !saved) return fail(PT_SCAN_ERR_ARG, "scan: the backward needs the forward's saved states");
-  if (p.segs > 1 && !workspace) return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace");
   a.h0 = h0; a.len = lengths; a.d_h_last = d_h_last; a.d_c_last = d_c_last; a.d_h0 = d_h0;
   a.saved = (float*)saved;
-  a.agg = (float*)workspace;
-  return run(d, p, ts, a, true, (hipStream_t)stream);
+  return run(d, p, ts, a, workspace, true, (hipStream_t)stream);
 }
 
 int pt_scan_step(const pt_scan_desc* d, const pt_scan_view* x, const pt_scan_view* state, const pt_scan_view* y,

@@ -103,7 +103,8 @@ def _run(form, dtype, b, t, f, seed, h0=True, lengths=None, stack=2, want_seq=Tr
 @pytest.mark.parametrize("b,t,f", [
     (1, 1, 1), (2, 3, 5), (3, 8, 64), (2, 9, 130),     # one wave; one chunk
     (2, 37, 200), (1, 33, 127), (3, 129, 66),          # several waves, ragged chunks
-    (1, 700, 65), (2, 1025, 34), (1, 5000, 3),         # time cut over workgroups
+    (1, 129, 3), (1, 700, 65), (2, 1025, 34),          # the chain: chunks of a row in workgroups of their own
+    (1, 9001, 3), (70, 400, 40),                       # more chunks than a group; more than the card holds
     (520, 41, 256),                                    # many columns: the four-wave groups
 ])
 def test_sizes(form, dtype, b, t, f):
@@ -112,10 +113,10 @@ def test_sizes(form, dtype, b, t, f):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("form", list(GATES))
-@pytest.mark.parametrize("t,f", [(5, 70), (70, 6), (600, 130), (2049, 2)])
+@pytest.mark.parametrize("t,f", [(5, 70), (70, 6), (600, 130), (2049, 2), (8200, 3)])
 def test_row_ends(form, dtype, t, f):
     """Ends of 0, 1, around a chunk's, the whole row, and outside [0, T]."""
-    ends = torch.tensor([0, 1, min(t, 31), min(t, 129), t - 1, t, t + 7, -3])
+    ends = torch.tensor([0, 1, min(t, 31), min(t, 129), t - 1, t, t + 7, -3, min(t, 4096), min(t, 4097)])
     _run(form, dtype, len(ends), t, f, seed=t, lengths=ends)
     _run(form, dtype, len(ends), t, f, seed=t + 1, lengths=ends.to(torch.int32), h0=False)
 
@@ -288,6 +289,34 @@ def test_two_runs_agree_bit_for_bit_and_other_streams_do():
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+def test_two_chains_at_once():
+    """Long rows on two streams at the same time: each call has a chain of its own."""
+    from ptamd import scan
+    dev = _dev()
+    xs, want = [], []
+    for k in range(2):
+        gates, _ = _gates("leaky", (1, 6000 + 500 * k, 256), torch.bfloat16, 90 + k)
+        xs.append(torch.cat(gates, 2).to(dev).requires_grad_())
+    one = torch.ones((), device=dev)
+
+    def once(k):
+        y, h = scan.gated_scan(xs[k])
+        return [y.detach(), h.detach(), torch.autograd.grad(h.sum(), xs[k], one)[0]]
+
+    want = [once(k) for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(once(k))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k])), k
 
 
 @pytest.mark.parametrize("t,f", [(40, 64), (1500, 33)])

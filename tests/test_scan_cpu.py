@@ -31,9 +31,9 @@ def test_sizes_of_the_buffers():
     d.steps = 1
     assert lib.pt_scan_saved_bytes(ctypes.byref(d)) == 0
     assert lib.pt_scan_workspace_bytes(ctypes.byref(d)) == 0
-    long = scan.Desc(0, 1, 1, 1, 65536, 64)      # one tile of columns: time is cut over workgroups
-    work = lib.pt_scan_workspace_bytes(ctypes.byref(long))
-    assert 0 < work <= 64 * 64 * 8
+    long = scan.Desc(0, 1, 1, 1, 65536, 64)      # one tile of columns: time is cut over workgroups,
+    work = lib.pt_scan_workspace_bytes(ctypes.byref(long))   # a pair of f32 per chunk of 64 steps or more
+    assert 0 < work <= 256 + (65536 // 64) * 64 * 8 * 33 // 32
 
 
 @pytest.mark.parametrize("field,value,word", [
@@ -56,6 +56,7 @@ def test_bad_descriptors_are_refused(field, value, word):
 def test_bad_pointers_are_refused():
     lib = scan.load()
     d = scan.Desc(0, 0, 1, 1, 100000, 64)
+    assert lib.pt_scan_workspace_bytes(ctypes.byref(d)) > 0 and lib.pt_scan_saved_bytes(ctypes.byref(d)) > 0
     good = (scan.View * 4)(*[scan.View(4096, 0, 0, 64) for _ in range(4)])
     null = (scan.View * 4)(scan.View(4096, 0, 0, 64), scan.View(None, 0, 0, 64))
     odd = (scan.View * 4)(*[scan.View(4098, 0, 0, 64) for _ in range(4)])
@@ -66,7 +67,7 @@ def test_bad_pointers_are_refused():
 
     apart = (scan.View * 4)(scan.View(4096, 0, 0, 64), scan.View(4096, 0, 0, 128))
     assert fwd(apart) == 2 and b"strides" in lib.pt_scan_last_error()
-    for x, work, word in ((None, 8192, b"null"), (null, 8192, b"null"), (good, None, b"workspace"),
+    for x, work, word in ((None, 8192, b"null"), (null, 8192, b"null"), (good, None, b"workspace"), (good, 8196, b"aligned"),
                           (odd, 8192, b"aligned")):
         assert fwd(x, work) == 1 and word in lib.pt_scan_last_error()
     for saved, work, word in ((None, 8192, b"saved"), (4096, None, b"workspace")):
