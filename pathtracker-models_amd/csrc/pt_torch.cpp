@@ -133,10 +133,12 @@ bool merge(const std::vector<int64_t>& size, const std::vector<std::vector<int64
 }
 
 // How tensors of one shape (their strides differing) fold into [batch][channels]
-// [steps][inner], time at `dim` (-1: no time axis).  batch_first: the batch is
-// dimension 0 alone, as row ends need it.
+// [steps][inner], time at `dim` (-1: no time axis).  The batch is the first `lead`
+// of the other dimensions (row ends need dimension 0 alone, and forward and
+// backward, whose tensors may be laid out differently, have to agree on how the
+// columns are cut), or as many as it takes (-1).
 std::optional<Fold> fold(at::IntArrayRef sizes, int64_t dim, const std::vector<at::IntArrayRef>& strides,
-                         bool batch_first) {
+                         int64_t lead) {
   std::vector<int64_t> size;
   std::vector<std::vector<int64_t>> st(strides.size());
   Fold f;
@@ -147,7 +149,7 @@ std::optional<Fold> fold(at::IntArrayRef sizes, int64_t dim, const std::vector<a
     for (size_t i = 0; i < strides.size(); ++i) st[i].push_back(strides[i][k]);
   }
   for (size_t i = 0; i < strides.size(); ++i) f.views[i].st = dim < 0 ? 0 : strides[i][dim];
-  const size_t first = batch_first ? 1 : 0;
+  const size_t first = lead < 0 ? 0 : lead;
   size_t inner = size.size();
   f.n = 1;
   while (inner > first) {                // every trailing axis that all tensors hold densely
@@ -157,7 +159,7 @@ std::optional<Fold> fold(at::IntArrayRef sizes, int64_t dim, const std::vector<a
     f.n *= size[--inner];
   }
   std::vector<int64_t> bs, cs;
-  for (size_t cut = first; cut <= inner; ++cut)          // dimensions cut..inner-1: channels
+  for (size_t cut = first; cut <= (lead < 0 ? inner : first); ++cut)    // dimensions cut..inner-1: channels
     if (merge(size, st, 0, cut, f.b, bs) && merge(size, st, cut, inner, f.c, cs)) {
       for (size_t i = 0; i < st.size(); ++i) {
         f.views[i].sb = bs[i];
@@ -221,10 +223,10 @@ void alike(Gates& gates) {
 }
 
 // The common layout of tensors, and views with their pointers.
-std::optional<Fold> fold_of(const std::vector<const Tensor*>& ts, int64_t dim, bool batch_first) {
+std::optional<Fold> fold_of(const std::vector<const Tensor*>& ts, int64_t dim, int64_t lead) {
   std::vector<at::IntArrayRef> st;
   for (const Tensor* t : ts) st.push_back(t->strides());
-  auto f = fold(ts[0]->sizes(), dim, st, batch_first);
+  auto f = fold(ts[0]->sizes(), dim, st, lead);
   if (f)
     for (size_t i = 0; i < ts.size(); ++i) f->views[i].data = ts[i]->data_ptr();
   return f;
@@ -263,7 +265,7 @@ Scanned forward(Form form, int64_t dim, int64_t gate_dim, bool want_seq, const T
     std::vector<const Tensor*> ts;
     append(ts, gates);
     if (want_seq) ts.push_back(&r.y);
-    return fold_of(ts, dim, lengths.defined() || dim != 0);
+    return fold_of(ts, dim, dim != 0);
   };
   auto f = folded();
   if (!f) {                              // no common layout: dense copies have one
@@ -353,7 +355,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
       append(ts, gates);
       append(ts, dgates);
       if (dy.defined()) ts.push_back(&dy);
-      return fold_of(ts, dim, lengths.defined() || dim != 0);
+      return fold_of(ts, dim, dim != 0);
     };
     auto f = folded();
     if (!f) {
@@ -529,7 +531,7 @@ Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::stri
     append(ts, gates);
     ts.push_back(&s);
     ts.push_back(&y);
-    return fold_of(ts, -1, false);
+    return fold_of(ts, -1, -1);
   };
   auto f = folded();
   if (!f) {
@@ -635,9 +637,9 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
 }
 
 py::object py_fold(const std::vector<int64_t>& sizes, int64_t dim, const std::vector<std::vector<int64_t>>& strides,
-                   bool batch_first) {
+                   int64_t lead) {
   std::vector<at::IntArrayRef> st(strides.begin(), strides.end());
-  const auto f = fold(sizes, dim, st, batch_first);
+  const auto f = fold(sizes, dim, st, lead);
   if (!f) return py::none();
   py::list v;
   for (const auto& s : f->views) v.append(py::make_tuple(s.sb, s.sc, s.st));

@@ -191,6 +191,35 @@ def test_strides_and_alignment(dtype):
         _close(d, val["dgates"][k], bnd["dgates"][k], ("turned", k))
 
 
+@pytest.mark.parametrize("form", list(GATES))
+def test_layouts_that_lie_like_a_larger_batch(form):
+    """Batch and a further axis one behind the other in memory, the rest padded: row
+    ends stay those of the batch, and a backward whose dy lies differently finds the
+    forward's states."""
+    from ptamd import scan
+    dev = _dev()
+    gates, g = _gates(form, (4, 30, 6, 5, 8), torch.float32, 71)
+    ends = torch.tensor([30, 0, 17, 1])
+    val, bnd = scan_ref.walk(form, [_btf(v, 1) for v in gates], lengths=ends)
+    padded = []
+    for v in gates:
+        p = torch.full((30, 4, 6, 6, 9), math.nan, device=dev)[:, :, :, :5, :8].transpose(0, 1)
+        padded.append(p.copy_(v))
+    res = scan.gated_scan(padded, form=form, lengths=ends.to(dev), want_seq=False)
+    _close(res[1], val["h"], bnd["h"], "h_last")
+
+    shape = (300, 130, 2, 5)                 # time first
+    gates, g = _gates(form, shape, torch.float32, 73)
+    dy = torch.randn(shape, generator=g)
+    val, bnd = scan_ref.walk(form, [_btf(v, 0) for v in gates], dy=_btf(dy, 0))
+    xs = [v.to(dev).requires_grad_() for v in gates]
+    y = scan.gated_scan(xs, form=form, dim=0)[0]
+    _close(_btf(y, 0), val["y"], bnd["y"], "y")
+    apart = torch.full((300, 130, 3, 6), math.nan, device=dev)[:, :, :2, :5].copy_(dy)
+    for k, d in enumerate(torch.autograd.grad(y, xs, apart)):
+        _close(_btf(d.cpu(), 0), val["dgates"][k], bnd["dgates"][k], k)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("form", list(GATES))
 def test_what_stands_behind_a_row_is_never_used(form, dtype):

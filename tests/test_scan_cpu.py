@@ -161,3 +161,20 @@ def test_overlapping_states_are_seen():
     apart = scan.native().disjoint
     assert apart((4, 6), (6, 1)) and apart((4, 6), (1, 4)) and apart((1, 6), (0, 1)) and apart((4, 6), (100, 2))
     assert not apart((4, 6), (0, 1)) and not apart((4, 6), (3, 1))
+
+
+def test_fold_keeps_the_batch_apart():
+    """Row ends are read per batch row, and how the columns are cut decides where the
+    backward finds its states: no layout may take another axis into the batch."""
+    fold = scan.native().fold
+    # memory [T][B][P][Q + 1][N + 1]: B and P lie like one axis, P and Q do not
+    x = torch.empty(5, 4, 6, 6, 9)[:, :, :, :5, :8].transpose(0, 1)          # [B, T, P, Q, N]
+    assert fold(x.shape, 1, (x.stride(),), True) is None
+    dense = torch.empty(x.shape)
+    assert fold(x.shape, 1, (dense.stride(),), True)[0] == 4
+    # time first: the batch and P apart in one tensor, together in another
+    y = torch.empty(5, 4, 7, 9)[:, :, :6, :8]
+    assert fold(y.shape, 0, (y.stride(),), False) is None
+    assert fold(y.shape, 0, (torch.empty(y.shape).stride(),), False)[:2] == (1, 1)
+    # a step has neither: its columns may be cut anyhow
+    assert fold((4, 6, 5, 8), -1, (x.select(1, 0).stride(),), -1)[0] == 24
