@@ -694,7 +694,9 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
 //
 // Workgroups take numbers from a ticket, so whatever a workgroup waits for was
 // taken up before it and waits itself only for still earlier ones: every wait
-// ends, whatever order the card starts them in.  A pair is one 64-bit word that
+// ends, whatever order the card starts them in.  Every chunk publishes what a
+// later one could wait for, also behind its row's end, so that the waits do not
+// hang on what `lengths` holds either.  A pair is one 64-bit word that
 // is written once, so a reader sees none of it or all of it, and needs no fence:
 // nothing but the word is handed over.  NOT_YET is what no pair can be (its P
 // would be a NaN of a form that is never published).
@@ -722,6 +724,12 @@ __device__ __forceinline__ void publish(uint64_t* slot, float p, float q) {
 }
 __device__ __forceinline__ uint64_t peek(const uint64_t* slot) {
   return __hip_atomic_load(slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// A chunk behind its row's end: nobody uses its pair, nor the state after it.
+__device__ __forceinline__ void publish_idle(const Args& a, const Where& w, bool chunk, bool group) {
+  if (w.wave != 0 || !w.on) return;
+  if (chunk) publish(a.pairs + w.seg * a.cols_all + w.state, 1.f, 0.f);
+  if (group) publish(a.states + w.seg / GROUP * a.cols_all + w.state, 1.f, 0.f);
 }
 // The pair, from a first look at it.  (Idle lanes look at column 0's, which is published as well.)
 __device__ __forceinline__ f32x2 await(const uint64_t* slot, uint64_t v) {
@@ -763,7 +771,9 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) 
   const bool seq = a.y != nullptr;
   char* yp = seq ? a.y + w.base(a.ys, t0) : nullptr;
   const uint32_t yo = seq ? w.lane_off(a.ys, sizeof(T)) : 0;
-  if (t_beg >= w.end) {                  // behind the row's end: nobody waits for this chunk
+  const bool more = w.seg + 1 < a.segs, hands_on = more && (w.seg + 1) % GROUP == 0;
+  if (t_beg >= w.end) {                  // behind the row's end
+    publish_idle(a, w, more, hands_on);
     const T none[L] = {};
     if (seq && w.on) store_steps(none, yp, a.ys.t, yo, 0, room);
     if (w.seg == 0 && w.wave == 0) last_states<FORM>(a, w, a.h0 ? a.h0[w.state] : 0.f);
@@ -785,7 +795,6 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) 
   pq[w.wave][w.lane] = f.piece();
   lds_barrier();
   const int first = w.seg & -GROUP, group = w.seg / GROUP;
-  const bool more = t_beg + CH < w.end;                 // a later chunk waits for this one
   f32x2 own = {1.f, 0.f};                               // wave 0: the chunk's pair
   if (w.wave == 0) {
 #pragma unroll
@@ -811,8 +820,8 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) 
   }
   if (w.wave == 0) {
     const float after = __builtin_fmaf(own[0], c, own[1]);
-    if (more && (w.seg + 1) % GROUP == 0 && w.on) publish(a.states + group * a.cols_all + w.state, 1.f, after);
-    if (!more) last_states<FORM>(a, w, after);
+    if (hands_on && w.on) publish(a.states + group * a.cols_all + w.state, 1.f, after);
+    if (t_beg + CH >= w.end) last_states<FORM>(a, w, after);
   }
   for (int k = 0; k < w.wave; ++k) {
     const f32x2 e = pq[k][w.lane];
@@ -838,7 +847,8 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_BWD, 4) 
   char* dp[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) dp[g] = a.dx[g] + d_at;
-  if (t_beg >= w.end) {                  // behind the row's end: nobody waits for this chunk
+  if (t_beg >= w.end) {                  // behind the row's end
+    publish_idle(a, w, w.seg > 0, w.seg > 0 && w.seg % GROUP == 0);
     const T none[L] = {};
 #pragma unroll
     for (int g = 0; g < G; ++g)
