@@ -184,6 +184,23 @@ bool disjoint(at::IntArrayRef sizes, at::IntArrayRef strides) {
   return true;
 }
 
+// The bytes from a tensor's first element to its last.
+std::pair<uintptr_t, uintptr_t> span_of(const Tensor& t) {
+  int64_t reach = 1;
+  for (int64_t k = 0; k < t.dim(); ++k) reach += (t.size(k) - 1) * t.stride(k);
+  const uintptr_t at = (uintptr_t)t.data_ptr();
+  return {at, at + (uintptr_t)reach * t.element_size()};
+}
+bool meet(const Tensor& a, const Tensor& b) {
+  const auto x = span_of(a), y = span_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+// What autograd has to know of a tensor that a kernel wrote in place.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 bool expanded(const Tensor& t) {
   for (int64_t k = 0; k < t.dim(); ++k)
     if (t.stride(k) == 0 && t.size(k) > 1) return true;
@@ -524,6 +541,8 @@ Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::stri
   TORCH_CHECK_VALUE(disjoint(state.sizes(), state.strides()),
                     "state's elements share memory: it cannot be updated in place");
   Gates gates = t.gate_dim >= 0 ? chunks(t.xs[0], form.gates, t.gate_dim) : t.xs;
+  for (auto& g : gates)                  // gates in the state's own memory: read before it is written
+    if (meet(g, state)) g = g.clone(at::MemoryFormat::Contiguous);
   alike(gates);
   Tensor s = state;
   auto folded = [&] {
@@ -543,6 +562,7 @@ Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::stri
   check_scan(lib.scan_step(&d, f->views.data(), &f->views[form.gates], &f->views[form.gates + 1],
                            stream_of<pt_scan_stream_t>(y)));
   if (s.data_ptr() != state.data_ptr()) state.copy_(s);
+  else written(state);
   return y;
 }
 
@@ -632,6 +652,8 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
     check_clip(lib.clip_grads(table.data(), n, code, max_norm, (float*)norm.data_ptr(), work.data_ptr(), stream));
   else
     check_clip(lib.clip_norm(table.data(), n, code, (float*)norm.data_ptr(), work.data_ptr(), stream));
+  if (scale)
+    for (size_t i = 0; i < grads.size(); ++i) written(out ? (*out)[i] : grads[i]);
   for (auto& [o, d] : back) o.copy_(d);
   return norm;
 }

@@ -105,10 +105,11 @@ def clip_grads(grads, max_norm, *, norm_type=2.0, out=None):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Clip the gradients of ``parameters`` (one or several) in place; returns
     their norm before (reference utils/misc_functions.py:48-69).  Parameters
-    without a gradient are left out."""
+    without a gradient are left out; one listed twice is refused (its gradient
+    would be scaled twice)."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads, norm_type = [p.grad for p in parameters if p.grad is not None], float(norm_type)
     if error_if_nonfinite:
         norm = grad_norm(grads, norm_type)
         if not math.isfinite(float(norm)):

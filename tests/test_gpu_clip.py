@@ -224,3 +224,26 @@ def test_parameters_of_a_model_as_the_reference_clips_them():
     assert m[2].bias.grad is None
     one = clip.clip_grad_norm_(params[0], 100.0)
     assert abs(float(one) - _norm([params[0].grad], 2.0)) <= float(one) * 2 * U
+
+
+def test_clipping_tells_autograd_that_it_wrote():
+    from ptamd import clip
+    dev = _dev()
+    w = torch.ones(8, device=dev, requires_grad=True)
+    for grads, out in (([torch.ones(8, device=dev)], None), ([torch.ones(16, device=dev)[::2]], None),
+                       ([torch.ones(8, device=dev)], [torch.ones(8, device=dev)])):
+        loss = (w * (out or grads)[0]).sum()
+        clip.grad_norm(grads)
+        clip.clip_grads(grads, 0.5, out=out)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+
+
+def test_a_parameter_listed_twice_is_refused():
+    from ptamd import clip
+    p = torch.nn.Parameter(torch.ones(8, device=_dev()))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(clip.PtClipError, match="shares memory"):
+        clip.clip_grad_norm_([p, p], 1.0)
+    assert torch.equal(p.grad, torch.ones_like(p))
+    assert abs(float(clip.clip_grad_norm_([p], 100.0, norm_type="inf")) - 1.0) <= U

@@ -440,6 +440,35 @@ def test_a_prompt_continued_step_by_step(form):
     _close(state, val["c"], bnd["c"], "state")
 
 
+@pytest.mark.parametrize("form", list(GATES))
+def test_step_with_the_state_inside_the_gates(form):
+    """Overlapping memory: every gate is read before the state is written."""
+    from ptamd import scan
+    dev = _dev()
+    n = GATES[form]
+    buf = torch.randn(3, (n + 1) * 700, generator=torch.Generator().manual_seed(5)).to(dev)
+    x, state = buf[:, :n * 700], buf[:, 350:1050]
+    want_state = state.clone()
+    want = scan.gated_scan_step(x.clone(), want_state, form=form)
+    y = scan.gated_scan_step(x, state, form=form)
+    assert torch.equal(y, want) and torch.equal(state, want_state)
+
+
+def test_a_step_tells_autograd_that_it_wrote():
+    from ptamd import scan
+    dev = _dev()
+    w = torch.ones(2, 4, device=dev, requires_grad=True)
+    for state in (torch.ones(2, 4, device=dev), torch.ones(2, 8, device=dev)[:, ::2]):
+        out = (w * state).sum()
+        scan.gated_scan_step(torch.zeros(2, 8, device=dev), state)
+        with pytest.raises(RuntimeError, match="inplace"):
+            out.backward()
+    with torch.inference_mode():
+        state = torch.ones(2, 4, device=dev)
+        assert float(scan.gated_scan_step(torch.zeros(2, 8, device=dev), state).sum()) == 4.0
+        assert float(state.sum()) == 4.0
+
+
 def test_empty_and_refused_calls():
     from ptamd import scan
     dev = _dev()
