@@ -222,8 +222,9 @@ __device__ __forceinline__ void load_steps(T (&r)[L], const char* p, int64_t st,
   } else {
 #pragma unroll
     for (int l = 0; l < L; ++l, p += st) {
-      r[l] = (T)0.f;
-      if (l < live) r[l] = *(const gval<T>*)(scalar(p) + offset32(off));
+      T v = (T)0.f;
+      if (l < live) v = *(const gval<T>*)(scalar(p) + offset32(off));
+      r[l] = v;
     }
   }
 }
@@ -243,7 +244,9 @@ __device__ __forceinline__ void store_steps(const T (&r)[L], char* p, int64_t st
 }
 
 // Registers whose contents no longer matter (else a loop that loads them in one
-// branch copies the old contents in the other).
+// branch copies the old contents in the other).  Written in front of that branch:
+// in its else, the stores of both were merged to one of a chosen address, and the
+// array lay in scratch memory.
 template <typename T, int L> __device__ __forceinline__ void forget(T (&r)[L]) {
 #pragma unroll
   for (int l = 0; l < L; ++l) asm("" : "=v"(r[l]));
@@ -296,11 +299,10 @@ template <int FORM, typename T, int L> struct Fwd {
       asm volatile("" : "+v"(A[l]), "+v"(B[l]));        // (one after the other, not all at once)
     }
     if constexpr (LSTM) {
+      forget(O);
       if (out_here) {
 #pragma unroll
         for (int l = 0; l < L; ++l) O[l] = logistic<ACC>(as_f32(raw[3][l])).s;
-      } else {
-        forget(O);
       }
     }
     settle(A);
@@ -387,8 +389,8 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
 #pragma unroll
     for (int g = 0; g < (LSTM ? 3 : 2); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, w.end - t0);
     if constexpr (LSTM) {                               // o is wanted for y, or at the row's last step
+      forget(raw[3]);
       if (out_in(t0)) load_steps(raw[3], xp[3], a.xs.t, xo, w.end - t0);
-      else forget(raw[3]);
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) xp[g] += x_step;
@@ -468,6 +470,8 @@ template <int FORM, typename T, int L> struct Bwd {
       }
     }
     if constexpr (!LEAKY) {
+      forget(O);
+      forget(OP);
       if (enters) {
 #pragma unroll
         for (int l = 0; l < L; ++l) {
@@ -475,9 +479,6 @@ template <int FORM, typename T, int L> struct Bwd {
           O[l] = g.s;
           OP[l] = g.p;
         }
-      } else {
-        forget(O);
-        forget(OP);
       }
       settle(B);
       settle(K2);
@@ -523,7 +524,6 @@ template <int FORM, typename T, int L> struct Bwd {
         c = __builtin_fmaf(A[l], c, s * n);
       }
     } else {
-      T out[L];
       if (enters) {
         if (a.d_h_last && t0 < w.end && w.end - t0 <= L) {
           const float e = a.d_h_last[w.state];
@@ -537,7 +537,7 @@ template <int FORM, typename T, int L> struct Bwd {
           c = __builtin_fmaf(A[l], c, B[l]);
           float d;
           const float th = tanh_d<ACC>(c, d);
-          out[l] = (T)(D[l] * th * OP[l]);
+          OP[l] *= D[l] * th;
           D[l] *= O[l] * d;
         }
       } else {
@@ -545,27 +545,33 @@ template <int FORM, typename T, int L> struct Bwd {
         for (int l = 0; l < L; ++l) {
           K1[l] *= c;
           c = __builtin_fmaf(A[l], c, B[l]);
-          out[l] = (T)0.f;
+          OP[l] = 0.f;
         }
       }
+      settle(OP);                        // (16-bit values made in both branches went through scratch memory)
+      T out[L];
+#pragma unroll
+      for (int l = 0; l < L; ++l) out[l] = (T)OP[l];
       if (w.on) store_steps(out, dp3, a.ds.t, dof, live, room);
     }
   }
   // The other gates' gradients, with g coming from behind; returns what leaves.
   __device__ __forceinline__ float finish(const Args& a, const Where& w, float g, int live, int room,
                                           char* const (&dp)[G], uint32_t dof) {
-    T out[3][L];
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
-      const float t = D[l] + g;
-      out[0][l] = (T)(t * K0[l]);
-      out[1][l] = (T)(t * K1[l]);
-      if constexpr (!LEAKY) out[2][l] = (T)(t * K2[l]);
-      g = A[l] * t;
+      D[l] += g;
+      g = A[l] * D[l];
     }
+    auto give = [&](const float (&k)[L], char* p) {
+      T out[L];
 #pragma unroll
-    for (int k = 0; k < (LEAKY ? 2 : 3); ++k)
-      if (w.on) store_steps(out[k], dp[k], a.ds.t, dof, live, room);
+      for (int l = 0; l < L; ++l) out[l] = (T)(D[l] * k[l]);
+      if (w.on) store_steps(out, p, a.ds.t, dof, live, room);
+    };
+    give(K0, dp[0]);
+    give(K1, dp[1]);
+    if constexpr (!LEAKY) give(K2, dp[2]);
     return g;
   }
 };
@@ -617,8 +623,8 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
 #pragma unroll
     for (int g = 0; g < (LEAKY ? 2 : 3); ++g) load_steps(raw[g], xp[g], a.xs.t, xo, live);
     if constexpr (!LEAKY) {
+      forget(raw[3]);
       if (enters_in(a, w, t0, L)) load_steps(raw[3], xp[3], a.xs.t, xo, live);
-      else forget(raw[3]);
     }
     if (has_dy) load_steps(rdy, yp, a.ys.t, yo, live);
     const float* s = tc > 0 ? a.saved + (tc / CH - 1) * a.cols_all : a.h0;
@@ -786,8 +792,8 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) 
 #pragma unroll
   for (int g = 0; g < (LSTM ? 3 : 2); ++g) load_steps(raw[g], a.x[g] + x_at, a.xs.t, xo, live);
   if constexpr (LSTM) {
+    forget(raw[3]);
     if (out_here) load_steps(raw[3], a.x[3] + x_at, a.xs.t, xo, live);
-    else forget(raw[3]);
   }
   Fwd<FORM, T, L> f;
   f.make(raw, out_here);
@@ -863,8 +869,8 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_BWD, 4) 
 #pragma unroll
   for (int g = 0; g < (LEAKY ? 2 : 3); ++g) load_steps(raw[g], a.x[g] + x_at, a.xs.t, xo, live);
   if constexpr (!LEAKY) {
+    forget(raw[3]);
     if (enters) load_steps(raw[3], a.x[3] + x_at, a.xs.t, xo, live);
-    else forget(raw[3]);
   }
   if (has_dy) load_steps(rdy, a.y + w.base(a.ys, t0), a.ys.t, w.lane_off(a.ys, sizeof(T)), live);
   const float* s = w.seg > 0 ? a.saved + (w.seg - 1) * a.cols_all : a.h0;
