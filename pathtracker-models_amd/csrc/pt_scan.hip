@@ -1013,11 +1013,11 @@ Plan plan_of(const pt_scan_desc* d) {
   return p;
 }
 
-// The chain's scratch: the ticket, a pair per chunk (of the backward: the most),
-// a state per group of chunks.
-size_t chain_bytes(const pt_scan_desc* d, const Plan& p) {
-  const int64_t words = (p.nchunks + (p.nchunks + GROUP - 1) / GROUP) * d->batch * d->channels * d->inner;
-  return p.W ? 0 : CHAIN_HEAD + ((size_t)words * sizeof(uint64_t) + 15) / 16 * 16;
+// The chain's scratch for `segs` chunks: the ticket, a pair per chunk, a state per
+// group of chunks.
+size_t chain_bytes(const pt_scan_desc* d, int64_t segs) {
+  const int64_t words = (segs + (segs + GROUP - 1) / GROUP) * d->batch * d->channels * d->inner;
+  return CHAIN_HEAD + ((size_t)words * sizeof(uint64_t) + 15) / 16 * 16;
 }
 
 // Strides of axes of one element never count: 0, so that they cannot spoil the alignment.
@@ -1118,8 +1118,8 @@ int run(const pt_scan_desc* d, const Plan& p, const Tensors& ts, Args& a, void* 
       return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace, aligned to 16 bytes");
     a.ticket = (uint32_t*)workspace;
     a.pairs = (uint64_t*)((char*)workspace + CHAIN_HEAD);
-    a.states = a.pairs + p.nchunks * a.cols_all;
-    const int64_t n = (int64_t)(chain_bytes(d, p) / 16);
+    a.states = a.pairs + a.segs * a.cols_all;
+    const int64_t n = (int64_t)(chain_bytes(d, a.segs) / 16);
     hipLaunchKernelGGL(k_chain_clear, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, s,
                        (vec<uint32_t, 4>*)workspace, n);
   }
@@ -1143,7 +1143,8 @@ size_t pt_scan_saved_bytes(const pt_scan_desc* d) {
 
 size_t pt_scan_workspace_bytes(const pt_scan_desc* d) {
   if (check(d)) return 0;
-  return chain_bytes(d, plan_of(d));
+  const Plan p = plan_of(d);
+  return p.W ? 0 : chain_bytes(d, p.nchunks);          // the backward's chunks: the most
 }
 
 int pt_scan_forward(const pt_scan_desc* d, const pt_scan_view* x, const float* h0, const int64_t* lengths,
