@@ -361,7 +361,15 @@ template <int FORM> __device__ __forceinline__ void last_states(const Args& a, c
   if (a.h_last && FORM == PT_SCAN_LSTM && w.end == 0) a.h_last[w.state] = 0.f;
 }
 
-// Forward, a workgroup walking a column tile's whole row.
+// Forward, a workgroup walking a column tile's whole row; each chunk's loads are
+// sent off before the one in front of it is finished.  Bound by memory where there
+// are columns enough: leaky f32, 32 clips of 64 frames of 32 x 32 x 32 (805 MB) in
+// 159 us, 5.1 TB/s (a copy of 4 GiB reaches 4.8).  For 16 bits the arithmetic is
+// nearly as long as the loads: lstm bf16, 64 clips of 64 frames of 25 x 32 x 32
+// without y (629 MB), 155 us, 4.1 TB/s, with the vector unit busy for three
+// quarters of it.  Of rows of unequal length the longest decides, where a
+// compute unit has one: leaky bf16 8 x 2048 x 2048, 68% of the steps live,
+// 40 us, 3.9 TB/s.
 template <int FORM, typename T, int W>
 __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
   constexpr int G = gates_of<FORM>(), L = 2 * back_steps<FORM>(), CH = W * L;
@@ -588,7 +596,11 @@ template <int FORM> __device__ __forceinline__ float end_gradient(const Args& a,
   return end ? end[w.state] : 0.f;
 }
 
-// Backward, a workgroup walking a column tile's whole row from its end.
+// Backward, a workgroup walking a column tile's whole row from its end.  Each
+// chunk is walked twice, both times from registers: forward from the kept state,
+// then back.  The shapes of the forward: leaky f32 (1342 MB) 261 us, 5.1 TB/s; lstm
+// bf16 (1468 MB) 334 us, 4.4 TB/s; leaky bf16 of unequal rows (271 MB) 78 us,
+// 3.5 TB/s.
 template <int FORM, typename T, int W>
 __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
   constexpr int G = gates_of<FORM>(), L = back_steps<FORM>(), CH = W * L;
@@ -706,11 +718,22 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
 // is written once, so a reader sees none of it or all of it, and needs no fence:
 // nothing but the word is handed over.  NOT_YET is what no pair can be (its P
 // would be a NaN of a form that is never published).
+//
+// A chunk is loaded, joined and stored by one workgroup that does nothing else, so
+// that the memory waits for the joins at times: leaky bf16, 16384 steps of 2048
+// columns (201 MB), 57 us, 3.5 TB/s; lstm bf16, 2 rows of 8192 steps of 512
+// (84 and 151 MB), forward 34 us and backward 53 us, 2.5 and 2.8 TB/s.  Reading the
+// sequence twice instead (every chunk's pair, then the walk) took, at 16384 steps
+// of 2048 columns, for leaky f32 128 us and in the backward 194, against 95 and
+// 132 here; for lstm bf16 128 and 248, against 113 and 193.  A workgroup that
+// sends off its next chunk's loads before it joins is slower (leaky bf16 92 us):
+// loads return in order, so the join then waits for the next chunk too.
 
 constexpr uint64_t NOT_YET = ~(uint64_t)0;
 constexpr int CHAIN_HEAD = 256;          // bytes of the ticket, in front of the pairs
 
-// The ticket to 0 and every pair to NOT_YET, `n` times 16 bytes.
+// The ticket to 0 and every pair to NOT_YET, `n` times 16 bytes (2 to 4 us; a kernel,
+// as a memory operation recorded into a graph is not safe to replay here).
 __global__ __launch_bounds__(256) void k_chain_clear(vec<uint32_t, 4>* p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
     p[i] = i < CHAIN_HEAD / 16 ? (vec<uint32_t, 4>)(0u) : (vec<uint32_t, 4>)(~0u);
@@ -767,6 +790,7 @@ __device__ __forceinline__ f32x2 join(const uint64_t* slot, int64_t step, int co
   return e;
 }
 
+// Forward: reduce, publish, join what lies before, walk.
 template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) void k_chain_fwd(Args a) {
   constexpr int W = CHAIN_FWD, G = gates_of<FORM>(), L = chain_steps<FORM>(), CH = W * L;
   constexpr bool LSTM = FORM == PT_SCAN_LSTM;
@@ -839,6 +863,8 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_FWD, 4) 
   f.finish(a, w, c, t0, live, room, seq, out_here, yp, yo);
 }
 
+// Backward: the states from the one kept at the chunk's start, then as the forward
+// from the far end.
 template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_BWD, 4) void k_chain_bwd(Args a) {
   constexpr int W = CHAIN_BWD, G = gates_of<FORM>(), L = chain_steps<FORM>(), CH = W * L;
   constexpr bool LEAKY = FORM == PT_SCAN_LEAKY;
@@ -925,7 +951,9 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_BWD, 4) 
   b.finish(a, w, g, live, room, dp, dof);
 }
 
-// One step: element-wise, one lane per V columns.
+// One step: element-wise, 16 bytes of the gates a lane where alignment allows.  Bound
+// by memory (lstm f32, 64 x 25600, 45.9 MB: 10.2 us, 4.5 TB/s) and by the launch for
+// one token (leaky bf16, 1 x 2048: 2.4 us on the device, 6.3 us a call).
 template <int FORM, typename T, int V>
 __global__ __launch_bounds__(256) void k_scan_step(Args a, char* state, Strides ss) {
   constexpr int G = gates_of<FORM>();
@@ -995,7 +1023,9 @@ struct Plan {
 //   129 .. 256    16 waves: one workgroup a compute unit (180 tiles: 81 us, 136
 //                 with 4, 108 with 8).
 //   up to 128     the chain, from more than one of its forward's chunks on; else 8
-//                 waves.
+//                 waves.  (4096 steps of leaky bf16, forward and backward: 64
+//                 tiles 42 and 47 us, 66 and 107 with 16 waves; 128 tiles 66 and
+//                 93, 67 and 136; 256 tiles 127 and 176, 95 and 147.)
 // Up to 4 L steps fit a chunk of 4 waves, up to L steps one wave.
 Plan plan_of(const pt_scan_desc* d) {
   Plan p;

@@ -247,3 +247,19 @@ def test_a_parameter_listed_twice_is_refused():
         clip.clip_grad_norm_([p, p], 1.0)
     assert torch.equal(p.grad, torch.ones_like(p))
     assert abs(float(clip.clip_grad_norm_([p], 100.0, norm_type="inf")) - 1.0) <= U
+
+
+def test_a_tensor_of_more_than_2_31_elements():
+    """It takes several entries of the pointer table; values around their seams."""
+    from ptamd import clip
+    n = 2 ** 31 + 12_345
+    g = torch.zeros(n, dtype=torch.bfloat16, device=_dev())
+    at = [0, 2 ** 28 - 1, 2 ** 28, 2 ** 31 - 1, 2 ** 31, n - 1]
+    for i in at:
+        g[i] = 2.0
+    norm = clip.clip_grads([g], 6.0 ** 0.5)
+    assert abs(float(norm) - 24.0 ** 0.5) <= 24.0 ** 0.5 * U
+    # k = sqrt(6) / (sqrt(24) + 1e-6): 2 k is below 1 by less than half a step of bf16
+    assert [float(g[i]) for i in at] == [1.0] * len(at)
+    g.abs_()
+    assert float(g.max()) == 1.0 and int(torch.count_nonzero(g)) == len(at)

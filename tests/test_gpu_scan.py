@@ -469,6 +469,44 @@ def test_a_step_tells_autograd_that_it_wrote():
         assert float(state.sum()) == 4.0
 
 
+@pytest.mark.parametrize("t,f", [(600_000, 2048), (60_000, 20_480)])
+def test_offsets_past_32_bits(t, f):
+    """4.9 GB of gates in one row (chunks of a row in workgroups of their own, and a
+    workgroup walking it): both ends as scans of their own give them.
+
+    A state is a mean of n's under weights that fall off fast: at most some 64
+    roundings of 2^-24 of max |n| < 7 count, 3e-5; the gradients' factors are G < 30
+    and |n - c| < 14, with s(z) s(-z) <= 1/4: 64 2^-24 30 14 / 4 < 5e-4.  bf16
+    outputs are off by half a step, 2^-8, on either side."""
+    from ptamd import scan
+    g = torch.Generator(device=_dev()).manual_seed(t)
+    x = torch.randn(1, t, 2 * f, generator=g, device=_dev(), dtype=torch.bfloat16)
+    dy = torch.randn(1, t, f, generator=g, device=_dev(), dtype=torch.bfloat16)
+    x.requires_grad_()
+    y, h = scan.gated_scan(x)
+    dx, = torch.autograd.grad(y, x, dy)
+    y, h, x = y.detach(), h.detach(), x.detach()
+    k = 1000
+
+    def same(got, want, tol):
+        assert bool(((got.float() - want.float()).abs() <= 2 ** -7 * want.float().abs() + tol).all())
+
+    def part(sl, h0):
+        xs = x[:, sl].clone().requires_grad_()
+        ys, hs = scan.gated_scan(xs, h0)
+        return ys.detach(), hs.detach(), torch.autograd.grad(ys, xs, dy[:, sl].clone())[0]
+
+    ys, _, dxs = part(slice(0, k), None)
+    same(y[:, :k], ys, 3e-5)
+    same(dx[:, :k // 2], dxs[:, :k // 2], 5e-4)
+    with torch.no_grad():
+        before = scan.gated_scan(x[:, :t - k], want_seq=False)[1]
+    ys, hs, dxs = part(slice(t - k, t), before)
+    same(y[:, t - k:], ys, 3e-5)
+    same(h, hs, 3e-5)
+    same(dx[:, t - k:], dxs, 5e-4)
+
+
 def test_empty_and_refused_calls():
     from ptamd import scan
     dev = _dev()
