@@ -953,7 +953,7 @@ template <int FORM, typename T> __global__ __launch_bounds__(64 * CHAIN_BWD, 4) 
 
 // One step: element-wise, 16 bytes of the gates a lane where alignment allows.  Bound
 // by memory (lstm f32, 64 x 25600, 45.9 MB: 10.2 us, 4.5 TB/s) and by the launch for
-// one token (leaky bf16, 1 x 2048: 2.4 us on the device, 6.3 us a call).
+// one token (leaky bf16, 1 x 2048: 2.4 us on the device, 5.0 us a call).
 template <int FORM, typename T, int V>
 __global__ __launch_bounds__(256) void k_scan_step(Args a, char* state, Strides ss) {
   constexpr int G = gates_of<FORM>();

@@ -108,21 +108,23 @@ int type_code(at::ScalarType t) {
 
 // ------------------------------------------------------------------ layouts
 
+using Dims = at::DimVector;
+constexpr size_t KINDS = 4;              // kinds of tensors of a call (gates, their gradients, y): strides differ
+
 struct Fold {
   int64_t b, c, n;
-  std::vector<pt_scan_view> views;       // strides; no pointers yet
+  pt_scan_view views[KINDS];             // strides; no pointers yet
 };
 
-// Dimensions lo..hi-1 as one axis of every tensor: its size and strides.
+// Dimensions lo..hi-1 as one axis of every kind: its size and strides.
 // Axes of one element drop out.
-bool merge(const std::vector<int64_t>& size, const std::vector<std::vector<int64_t>>& st, size_t lo, size_t hi,
-           int64_t& n, std::vector<int64_t>& out) {
+bool merge(const Dims& size, const Dims* st, size_t kinds, size_t lo, size_t hi, int64_t& n, int64_t (&out)[KINDS]) {
   n = 1;
-  out.assign(st.size(), 0);
+  std::fill(std::begin(out), std::end(out), 0);
   bool first = true;
   for (size_t k = hi; k-- > lo;) {
     if (size[k] == 1) continue;
-    for (size_t i = 0; i < st.size(); ++i) {
+    for (size_t i = 0; i < kinds; ++i) {
       if (first) out[i] = st[i][k];
       else if (st[i][k] != out[i] * n) return false;
     }
@@ -137,31 +139,30 @@ bool merge(const std::vector<int64_t>& size, const std::vector<std::vector<int64
 // of the other dimensions (row ends need dimension 0 alone, and forward and
 // backward, whose tensors may be laid out differently, have to agree on how the
 // columns are cut), or as many as it takes (-1).
-std::optional<Fold> fold(at::IntArrayRef sizes, int64_t dim, const std::vector<at::IntArrayRef>& strides,
-                         int64_t lead) {
-  std::vector<int64_t> size;
-  std::vector<std::vector<int64_t>> st(strides.size());
+std::optional<Fold> fold(at::IntArrayRef sizes, int64_t dim, at::ArrayRef<at::IntArrayRef> strides, int64_t lead) {
+  const size_t kinds = strides.size();
+  TORCH_CHECK(kinds <= KINDS, "too many kinds of tensors");
+  Dims size, st[KINDS];
   Fold f;
-  f.views.resize(strides.size());
   for (size_t k = 0; k < sizes.size(); ++k) {
     if ((int64_t)k == dim) continue;
     size.push_back(sizes[k]);
-    for (size_t i = 0; i < strides.size(); ++i) st[i].push_back(strides[i][k]);
+    for (size_t i = 0; i < kinds; ++i) st[i].push_back(strides[i][k]);
   }
-  for (size_t i = 0; i < strides.size(); ++i) f.views[i].st = dim < 0 ? 0 : strides[i][dim];
+  for (size_t i = 0; i < kinds; ++i) f.views[i] = {nullptr, 0, 0, dim < 0 ? 0 : strides[i][dim]};
   const size_t first = lead < 0 ? 0 : lead;
   size_t inner = size.size();
   f.n = 1;
   while (inner > first) {                // every trailing axis that all tensors hold densely
     bool dense = true;
-    for (const auto& s : st) dense = dense && (size[inner - 1] == 1 || s[inner - 1] == f.n);
+    for (size_t i = 0; i < kinds; ++i) dense = dense && (size[inner - 1] == 1 || st[i][inner - 1] == f.n);
     if (!dense) break;
     f.n *= size[--inner];
   }
-  std::vector<int64_t> bs, cs;
+  int64_t bs[KINDS], cs[KINDS];
   for (size_t cut = first; cut <= (lead < 0 ? inner : first); ++cut)    // dimensions cut..inner-1: channels
-    if (merge(size, st, 0, cut, f.b, bs) && merge(size, st, cut, inner, f.c, cs)) {
-      for (size_t i = 0; i < st.size(); ++i) {
+    if (merge(size, st, kinds, 0, cut, f.b, bs) && merge(size, st, kinds, cut, inner, f.c, cs)) {
+      for (size_t i = 0; i < kinds; ++i) {
         f.views[i].sb = bs[i];
         f.views[i].sc = cs[i];
       }
@@ -230,27 +231,57 @@ Gates chunks(const Tensor& x, int gates, int64_t gate_dim) {
   return out;
 }
 
-// The gates with one set of strides, as the library reads them.
-void alike(Gates& gates) {
-  for (const auto& g : gates)
-    if (g.strides() != gates[0].strides()) {
-      for (auto& h : gates) h = h.contiguous();
+// The gates of a call as the library reads them: one shape, one set of strides,
+// a pointer each.  Of stacked gates no views are made (a token's call is short).
+struct Side {
+  Dims shape, strides;
+  void* p[4];
+  int count;
+  Gates hold;                            // copies that the pointers belong to
+
+  // stacked along gate_dim, or (-1) a tensor each; copied where their strides differ
+  Side(const Gates& xs, int gates, int64_t gate_dim) : count(gates) {
+    if (gate_dim < 0) {
+      take(xs);
       return;
     }
+    const Tensor& x = xs[0];
+    shape = Dims(x.sizes().begin(), x.sizes().end());
+    strides = Dims(x.strides().begin(), x.strides().end());
+    shape[gate_dim] /= gates;
+    const int64_t step = shape[gate_dim] * strides[gate_dim] * (int64_t)x.element_size();
+    for (int g = 0; g < gates; ++g) p[g] = (char*)x.data_ptr() + g * step;
+  }
+  void take(const Gates& xs) {
+    hold = xs;
+    for (const auto& g : xs)
+      if (g.strides() != xs[0].strides()) {
+        for (auto& h : hold) h = h.contiguous();
+        break;
+      }
+    shape = Dims(xs[0].sizes().begin(), xs[0].sizes().end());
+    strides = Dims(hold[0].strides().begin(), hold[0].strides().end());
+    for (int g = 0; g < count; ++g) p[g] = hold[g].data_ptr();
+  }
+  void views(const pt_scan_view& like, pt_scan_view* out) const {
+    for (int g = 0; g < count; ++g) {
+      out[g] = like;
+      out[g].data = p[g];
+    }
+  }
+};
+
+Gates apart(const Gates& xs, int gates, int64_t gate_dim) {
+  return gate_dim >= 0 ? chunks(xs[0], gates, gate_dim) : xs;
 }
 
-// The common layout of tensors, and views with their pointers.
-std::optional<Fold> fold_of(const std::vector<const Tensor*>& ts, int64_t dim, int64_t lead) {
-  std::vector<at::IntArrayRef> st;
-  for (const Tensor* t : ts) st.push_back(t->strides());
-  auto f = fold(ts[0]->sizes(), dim, st, lead);
-  if (f)
-    for (size_t i = 0; i < ts.size(); ++i) f->views[i].data = ts[i]->data_ptr();
-  return f;
+void dense_copies(Gates& gates) {
+  for (auto& g : gates) g = g.contiguous();
 }
 
-void append(std::vector<const Tensor*>& v, const Gates& g) {
-  for (const auto& t : g) v.push_back(&t);
+pt_scan_view at_data(pt_scan_view v, const Tensor& t) {
+  v.data = t.data_ptr();
+  return v;
 }
 
 std::vector<int64_t> without(at::IntArrayRef sizes, int64_t dim) {
@@ -271,32 +302,34 @@ struct Scanned {
 
 Scanned forward(Form form, int64_t dim, int64_t gate_dim, bool want_seq, const Tensor& lengths, const Tensor& h0,
                 const Gates& xs, bool keep) {
-  Gates gates = gate_dim >= 0 ? chunks(xs[0], form.gates, gate_dim) : xs;
-  alike(gates);
-  const c10::DeviceGuard guard(gates[0].device());
-  const auto opts = gates[0].options();
-  const auto end = without(gates[0].sizes(), dim);
+  const c10::DeviceGuard guard(xs[0].device());
+  const auto opts = xs[0].options().requires_grad(false);
+  Side x(xs, form.gates, gate_dim);
+  const auto end = without(x.shape, dim);
   Scanned r;
-  if (want_seq) r.y = at::empty(gates[0].sizes(), opts);
+  if (want_seq) r.y = at::empty(x.shape, opts);
   auto folded = [&] {
-    std::vector<const Tensor*> ts;
-    append(ts, gates);
-    if (want_seq) ts.push_back(&r.y);
-    return fold_of(ts, dim, dim != 0);
+    at::IntArrayRef st[] = {x.strides, want_seq ? r.y.strides() : at::IntArrayRef()};
+    return fold(x.shape, dim, at::ArrayRef<at::IntArrayRef>(st, want_seq ? 2 : 1), dim != 0);
   };
   auto f = folded();
   if (!f) {                              // no common layout: dense copies have one
-    for (auto& g : gates) g = g.contiguous();
+    Gates gates = apart(xs, form.gates, gate_dim);
+    dense_copies(gates);
+    x.take(gates);
     f = folded();
   }
-  const pt_scan_desc d{form.code, type_code(gates[0].scalar_type()), f->b, f->c, gates[0].size(dim), f->n};
+  pt_scan_view xv[4], yv;
+  x.views(f->views[0], xv);
+  if (want_seq) yv = at_data(f->views[1], r.y);
+  const pt_scan_desc d{form.code, type_code(xs[0].scalar_type()), f->b, f->c, x.shape[dim], f->n};
   r.h_last = at::empty(end, opts.dtype(at::kFloat));
   if (form.lstm()) r.c_last = at::empty(end, opts.dtype(at::kFloat));
-  if (keep) r.saved = bytes(lib.scan_saved(&d), gates[0]);
-  const Tensor work = bytes(lib.scan_work(&d), gates[0]);
-  check_scan(lib.scan_forward(&d, f->views.data(), ptr<float>(h0), ptr<int64_t>(lengths),
-                              want_seq ? &f->views[form.gates] : nullptr, ptr<float>(r.h_last), ptr<float>(r.c_last),
-                              ptr<void>(r.saved), ptr<void>(work), stream_of<pt_scan_stream_t>(gates[0])));
+  if (keep) r.saved = bytes(lib.scan_saved(&d), xs[0]);
+  const Tensor work = bytes(lib.scan_work(&d), xs[0]);
+  check_scan(lib.scan_forward(&d, xv, ptr<float>(h0), ptr<int64_t>(lengths), want_seq ? &yv : nullptr,
+                              ptr<float>(r.h_last), ptr<float>(r.c_last), ptr<void>(r.saved), ptr<void>(work),
+                              stream_of<pt_scan_stream_t>(xs[0])));
   return r;
 }
 
@@ -356,47 +389,44 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
     if (dy.defined() && expanded(dy)) dy = dy.contiguous();      // (of a sum, a mean) no dense axis
     if (dh.defined()) dh = dh.contiguous();
     if (dc.defined()) dc = dc.contiguous();
-    Tensor whole;
-    Gates gates, dgates;
-    if (gate_dim >= 0) {
-      gates = chunks(xs[0], form.gates, gate_dim);
-      whole = at::empty_like(xs[0]);
-      dgates = chunks(whole, form.gates, gate_dim);
-    } else {
-      gates = xs;
-      alike(gates);
-      for (const auto& g : gates) dgates.push_back(at::empty_like(g));
-    }
+    Side x(xs, form.gates, gate_dim);
+    Gates dxs;                           // stacked as x is, or one a gate
+    if (gate_dim >= 0) dxs.push_back(at::empty_like(xs[0]));
+    else
+      for (const auto& g : x.hold) dxs.push_back(at::empty_like(g));
+    Side dx(dxs, form.gates, gate_dim);
     auto folded = [&] {
-      std::vector<const Tensor*> ts;
-      append(ts, gates);
-      append(ts, dgates);
-      if (dy.defined()) ts.push_back(&dy);
-      return fold_of(ts, dim, dim != 0);
+      at::IntArrayRef st[] = {x.strides, dx.strides, dy.defined() ? dy.strides() : at::IntArrayRef()};
+      return fold(x.shape, dim, at::ArrayRef<at::IntArrayRef>(st, dy.defined() ? 3 : 2), dim != 0);
     };
     auto f = folded();
-    if (!f) {
-      whole = Tensor();
-      for (int g = 0; g < form.gates; ++g) {
-        gates[g] = gates[g].contiguous();
-        dgates[g] = at::empty_like(gates[g]);
-      }
+    const bool copied = !f;
+    if (copied) {                        // no common layout: dense tensors have one
+      Gates gates = apart(xs, form.gates, gate_dim);
+      dense_copies(gates);
+      x.take(gates);
+      dxs.clear();
+      for (const auto& g : gates) dxs.push_back(at::empty_like(g));
+      dx.take(dxs);
       if (dy.defined()) dy = dy.contiguous();
       f = folded();
     }
-    const pt_scan_desc d{form.code, type_code(gates[0].scalar_type()), f->b, f->c, gates[0].size(dim), f->n};
+    pt_scan_view xv[4], dv[4], yv;
+    x.views(f->views[0], xv);
+    dx.views(f->views[1], dv);
+    if (dy.defined()) yv = at_data(f->views[2], dy);
+    const pt_scan_desc d{form.code, type_code(xs[0].scalar_type()), f->b, f->c, x.shape[dim], f->n};
     const Tensor dh0 = h0.defined() && h0.requires_grad() ? at::empty_like(h0) : Tensor();
-    const Tensor work = bytes(lib.scan_work(&d), gates[0]);
-    check_scan(lib.scan_backward(&d, f->views.data(), ptr<float>(h0), ptr<int64_t>(lengths),
-                                 dy.defined() ? &f->views[2 * form.gates] : nullptr, ptr<float>(dh), ptr<float>(dc),
-                                 ptr<void>(states), &f->views[form.gates], ptr<float>(dh0), ptr<void>(work),
-                                 stream_of<pt_scan_stream_t>(gates[0])));
+    const Tensor work = bytes(lib.scan_work(&d), xs[0]);
+    check_scan(lib.scan_backward(&d, xv, ptr<float>(h0), ptr<int64_t>(lengths), dy.defined() ? &yv : nullptr,
+                                 ptr<float>(dh), ptr<float>(dc), ptr<void>(states), dv, ptr<float>(dh0),
+                                 ptr<void>(work), stream_of<pt_scan_stream_t>(xs[0])));
     variable_list out(kArgs);
     out[6] = dh0;
     if (gate_dim >= 0) {
-      out[7] = whole.defined() ? whole : at::cat(dgates, gate_dim);
+      out[7] = copied ? at::cat(dxs, gate_dim) : dxs[0];
     } else {
-      for (int g = 0; g < form.gates; ++g) out[7 + g] = dgates[g];
+      for (int g = 0; g < form.gates; ++g) out[7 + g] = dxs[g];
     }
     return out;
   }
@@ -540,27 +570,27 @@ Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::stri
   if (y.numel() == 0) return y;
   TORCH_CHECK_VALUE(disjoint(state.sizes(), state.strides()),
                     "state's elements share memory: it cannot be updated in place");
-  Gates gates = t.gate_dim >= 0 ? chunks(t.xs[0], form.gates, t.gate_dim) : t.xs;
-  for (auto& g : gates)                  // gates in the state's own memory: read before it is written
-    if (meet(g, state)) g = g.clone(at::MemoryFormat::Contiguous);
-  alike(gates);
+  for (auto& v : t.xs)                   // gates in the state's own memory: read before it is written
+    if (meet(v, state)) v = v.clone(at::MemoryFormat::Contiguous);
+  Side gates(t.xs, form.gates, t.gate_dim);
   Tensor s = state;
   auto folded = [&] {
-    std::vector<const Tensor*> ts;
-    append(ts, gates);
-    ts.push_back(&s);
-    ts.push_back(&y);
-    return fold_of(ts, -1, -1);
+    at::IntArrayRef st[] = {gates.strides, s.strides(), y.strides()};
+    return fold(gates.shape, -1, st, -1);
   };
   auto f = folded();
   if (!f) {
-    for (auto& g : gates) g = g.contiguous();
+    Gates copies = apart(t.xs, form.gates, t.gate_dim);
+    dense_copies(copies);
+    gates.take(copies);
     s = state.contiguous();
     f = folded();
   }
+  pt_scan_view xv[4];
+  gates.views(f->views[0], xv);
+  const pt_scan_view sv = at_data(f->views[1], s), yv = at_data(f->views[2], y);
   const pt_scan_desc d{form.code, type_code(y.scalar_type()), f->b, f->c, 1, f->n};
-  check_scan(lib.scan_step(&d, f->views.data(), &f->views[form.gates], &f->views[form.gates + 1],
-                           stream_of<pt_scan_stream_t>(y)));
+  check_scan(lib.scan_step(&d, xv, &sv, &yv, stream_of<pt_scan_stream_t>(y)));
   if (s.data_ptr() != state.data_ptr()) state.copy_(s);
   else written(state);
   return y;
@@ -664,7 +694,7 @@ py::object py_fold(const std::vector<int64_t>& sizes, int64_t dim, const std::ve
   const auto f = fold(sizes, dim, st, lead);
   if (!f) return py::none();
   py::list v;
-  for (const auto& s : f->views) v.append(py::make_tuple(s.sb, s.sc, s.st));
+  for (size_t i = 0; i < st.size(); ++i) v.append(py::make_tuple(f->views[i].sb, f->views[i].sc, f->views[i].st));
   return py::make_tuple(f->b, f->c, f->n, v);
 }
 
