@@ -361,18 +361,18 @@ template <int FORM> __device__ __forceinline__ void last_states(const Args& a, c
   if (a.h_last && FORM == PT_SCAN_LSTM && w.end == 0) a.h_last[w.state] = 0.f;
 }
 
-// Forward, a workgroup walking a column tile's whole row; each chunk's loads are
-// sent off before the one in front of it is finished.  Bound by memory where there
-// are columns enough: leaky f32, 32 clips of 64 frames of 32 x 32 x 32 (805 MB) in
+// Forward, a workgroup walking a column tile's whole row, M times the backward's
+// steps a wave; each chunk's loads are sent off before the one in front of it is
+// finished.  Bound by memory where there are columns enough: leaky f32, 32 clips of 64 frames of 32 x 32 x 32 (805 MB) in
 // 159 us, 5.1 TB/s (a copy of 4 GiB reaches 4.8).  For 16 bits the arithmetic is
 // nearly as long as the loads: lstm bf16, 64 clips of 64 frames of 25 x 32 x 32
 // without y (629 MB), 155 us, 4.1 TB/s, with the vector unit busy for three
 // quarters of it.  Of rows of unequal length the longest decides, where a
 // compute unit has one: leaky bf16 8 x 2048 x 2048, 68% of the steps live,
 // 40 us, 3.9 TB/s.
-template <int FORM, typename T, int W>
+template <int FORM, typename T, int W, int M>
 __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
-  constexpr int G = gates_of<FORM>(), L = 2 * back_steps<FORM>(), CH = W * L;
+  constexpr int G = gates_of<FORM>(), L = M * back_steps<FORM>(), CH = W * L;
   constexpr bool LSTM = FORM == PT_SCAN_LSTM;
   // The waves' (P, q).  Two sets, used in turn: a wave writes a set again only
   // behind a barrier that every wave reaches after its last read of it, so one
@@ -438,8 +438,10 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_fwd(Args a) {
       }
       par ^= 1;
       // where the backward's chunks begin
-      if (a.saved && (w.wave == 0 || w.wave == W / 2) && t0 > 0 && t0 < a.T && w.on)
-        a.saved[(t0 / (CH / 2) - 1) * a.cols_all + w.state] = cin;
+      if constexpr (M == 2) {
+        if (a.saved && (w.wave == 0 || w.wave == W / 2) && t0 > 0 && t0 < a.T && w.on)
+          a.saved[(t0 / (CH / 2) - 1) * a.cols_all + w.state] = cin;
+      }
     }
     const float after = f.finish(a, w, cin, t0, live, room, seq, out_in(t0), yp, yo);
     if constexpr (W == 1) carry = after;
@@ -1067,9 +1069,16 @@ bool spans32(const pt_scan_desc* d, const pt_scan_view& v, int size) {
   return v.sc >= 0 && s < 2147483648.0;
 }
 
-template <int FORM, typename T, int W> void launch_rows(const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
-  if (bwd) hipLaunchKernelGGL((k_scan_bwd<FORM, T, W>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
-  else hipLaunchKernelGGL((k_scan_fwd<FORM, T, W>), dim3((unsigned)blocks), dim3(64 * W), 0, s, a);
+// The forward takes the backward's short chunk where that holds the whole row: of
+// twice the steps a wave, half the waves would have none (lstm bf16 64 x 16 x 4096:
+// 20 us, 13 with the short one; leaky f32 2 x 37 x 200: 5.0, 4.6).  Longer rows want
+// the long one (leaky bf16 4096 x 16384: 95 us, 107 with the short one).
+template <int FORM, typename T, int W>
+void launch_rows(const Plan& p, const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
+  const dim3 grid((unsigned)blocks), block(64 * W);
+  if (bwd) hipLaunchKernelGGL((k_scan_bwd<FORM, T, W>), grid, block, 0, s, a);
+  else if (p.nchunks == 1) hipLaunchKernelGGL((k_scan_fwd<FORM, T, W, 1>), grid, block, 0, s, a);
+  else if constexpr (W > 1) hipLaunchKernelGGL((k_scan_fwd<FORM, T, W, 2>), grid, block, 0, s, a);
 }
 
 template <int FORM, typename T> void launch_chain(const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
@@ -1081,10 +1090,10 @@ template <int FORM, typename T>
 int launch_w(const Plan& p, const Args& a, int64_t blocks, bool bwd, hipStream_t s) {
   switch (p.W) {
     case 0: launch_chain<FORM, T>(a, blocks, bwd, s); break;
-    case 1: launch_rows<FORM, T, 1>(a, blocks, bwd, s); break;
-    case 4: launch_rows<FORM, T, 4>(a, blocks, bwd, s); break;
-    case 8: launch_rows<FORM, T, 8>(a, blocks, bwd, s); break;
-    default: launch_rows<FORM, T, 16>(a, blocks, bwd, s);
+    case 1: launch_rows<FORM, T, 1>(p, a, blocks, bwd, s); break;
+    case 4: launch_rows<FORM, T, 4>(p, a, blocks, bwd, s); break;
+    case 8: launch_rows<FORM, T, 8>(p, a, blocks, bwd, s); break;
+    default: launch_rows<FORM, T, 16>(p, a, blocks, bwd, s);
   }
   return hipGetLastError() == hipSuccess ? 0 : fail(PT_SCAN_ERR_HIP, "scan: launch failed");
 }

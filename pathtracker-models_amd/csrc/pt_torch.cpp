@@ -632,7 +632,7 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
       TORCH_CHECK_TYPE(o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat, "an output of type ",
                        o.scalar_type(), " for a gradient of type ", g.scalar_type());
       if (o.device() != g.device()) raise(clip_error_type, "outputs are not on the gradients' device");
-      if (!disjoint(o.sizes(), o.strides()) && !dense(o))
+      if (!dense(o) && !disjoint(o.sizes(), o.strides()))
         raise(clip_error_type, "an output's elements share memory");
     }
   }
