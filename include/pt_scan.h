@@ -19,7 +19,8 @@
  * Conventions as pt_cell.h: caller-allocated device buffers, explicit stream,
  * 0 or PT_SCAN_ERR_* with a thread-local message, no state between calls.  No
  * call synchronises; every call can be captured into a graph.  Results do not
- * depend on timing: two runs agree bit for bit.
+ * depend on timing: two runs agree bit for bit.  What a call writes shares no
+ * memory with anything else that it is given.
  */
 #ifndef PT_SCAN_H
 #define PT_SCAN_H

@@ -375,6 +375,8 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
       out = run(form, dim, gate_dim, want_seq, lengths, h0, states, xs, grads);
     }
     if (at::GradMode::is_enabled()) {    // the gradients have no derivative of their own
+      for (auto& v : out)                // (of gradients that need none the error would leave no trace)
+        if (v.defined()) v = v.detach().set_requires_grad(true);
       auto err = std::make_shared<torch::autograd::DelayedError>(
           "gated_scan is differentiable once: its gradients have no derivative", (int)out.size());
       return (*err)(std::move(out));

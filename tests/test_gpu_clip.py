@@ -263,3 +263,16 @@ def test_a_tensor_of_more_than_2_31_elements():
     assert [float(g[i]) for i in at] == [1.0] * len(at)
     g.abs_()
     assert float(g.max()) == 1.0 and int(torch.count_nonzero(g)) == len(at)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+def test_so_many_partial_sums_that_they_are_added_in_a_launch_of_their_own(p):
+    from ptamd import clip
+    flat = torch.randn(1300, 32_768, generator=torch.Generator(device=_dev()).manual_seed(3), device=_dev())
+    before = flat.double()
+    want = float(torch.linalg.vector_norm(before, p))
+    norm = clip.clip_grads(list(flat), want / 8, norm_type=p)
+    assert abs(float(norm) - want) <= want * (U + 2 ** -29)
+    # k in 64 bits from a norm within 2^-29, the product rounded once
+    k = (want / 8) / (want + 1e-6)
+    assert bool(((flat.double() - before * k).abs() <= before.abs() * k * (U + 2 ** -28)).all())

@@ -469,6 +469,29 @@ def test_a_step_tells_autograd_that_it_wrote():
         assert float(state.sum()) == 4.0
 
 
+@pytest.mark.parametrize("t", [40, 900])
+@pytest.mark.parametrize("form,which", [("leaky", "y"), ("leaky", "h"), ("lstm", "y"), ("lstm", "h"), ("lstm", "c")])
+def test_one_output_alone_has_a_gradient(form, which, t):
+    """The others' gradients are absent, not zero tensors."""
+    gates, g = _gates(form, (2, t, 70), torch.bfloat16, t + len(which))
+    d = torch.randn((2, t, 70) if which == "y" else (2, 70), generator=g)
+    ends = torch.tensor([t, t // 3])
+    _check(form, gates, 1, stack=2, h0=torch.randn(2, 70, generator=g), lengths=ends,
+           **{"d" + which: d.to(torch.bfloat16) if which == "y" else d})
+
+
+def test_graphs_of_the_gradients():
+    """create_graph leaves the first gradients as they are and refuses the second."""
+    from ptamd import scan
+    dev = _dev()
+    x = torch.randn(2, 30, 16, device=dev, requires_grad=True)
+    want, = torch.autograd.grad(scan.gated_scan(x)[0].sum(), x)
+    got, = torch.autograd.grad(scan.gated_scan(x)[0].sum(), x, create_graph=True)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        got.sum().backward()
+
+
 @pytest.mark.parametrize("t,f", [(600_000, 2048), (60_000, 20_480)])
 def test_offsets_past_32_bits(t, f):
     """4.9 GB of gates in one row (chunks of a row in workgroups of their own, and a
