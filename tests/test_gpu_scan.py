@@ -106,6 +106,7 @@ def _run(form, dtype, b, t, f, seed, h0=True, lengths=None, stack=2, want_seq=Tr
     (1, 129, 3), (1, 700, 65), (2, 1025, 34),          # the chain: chunks of a row in workgroups of their own
     (1, 9001, 3), (70, 400, 40),                       # more chunks than a group; more than the card holds
     (520, 41, 256),                                    # many columns: the four-wave groups
+    (1000, 9, 3), (300, 140, 7), (9000, 3, 1),         # rows of few columns, side by side
 ])
 def test_sizes(form, dtype, b, t, f):
     _run(form, dtype, b, t, f, seed=b * 1000 + t)
@@ -208,16 +209,17 @@ def test_layouts_that_lie_like_a_larger_batch(form):
     res = scan.gated_scan(padded, form=form, lengths=ends.to(dev), want_seq=False)
     _close(res[1], val["h"], bnd["h"], "h_last")
 
-    shape = (300, 130, 2, 5)                 # time first
-    gates, g = _gates(form, shape, torch.float32, 73)
-    dy = torch.randn(shape, generator=g)
-    val, bnd = scan_ref.walk(form, [_btf(v, 0) for v in gates], dy=_btf(dy, 0))
-    xs = [v.to(dev).requires_grad_() for v in gates]
-    y = scan.gated_scan(xs, form=form, dim=0)[0]
-    _close(_btf(y, 0), val["y"], bnd["y"], "y")
-    apart = torch.full((300, 130, 3, 6), math.nan, device=dev)[:, :, :2, :5].copy_(dy)
-    for k, d in enumerate(torch.autograd.grad(y, xs, apart)):
-        _close(_btf(d.cpu(), 0), val["dgates"][k], bnd["dgates"][k], k)
+    for shape, dim in (((300, 130, 2, 5), 0), ((130, 300, 2, 5), 1), ((130, 2, 300, 5), 2)):
+        gates, g = _gates(form, shape, torch.float32, 73)
+        dy = torch.randn(shape, generator=g)
+        val, bnd = scan_ref.walk(form, [_btf(v, dim) for v in gates], dy=_btf(dy, dim))
+        xs = [v.to(dev).requires_grad_() for v in gates]
+        y = scan.gated_scan(xs, form=form, dim=dim)[0]
+        _close(_btf(y, dim), val["y"], bnd["y"], (dim, "y"))
+        wide = torch.full([n + 1 for n in shape], math.nan, device=dev)
+        apart = wide[tuple(slice(0, n) for n in shape)].copy_(dy)
+        for k, d in enumerate(torch.autograd.grad(y, xs, apart)):
+            _close(_btf(d.cpu(), dim), val["dgates"][k], bnd["dgates"][k], (dim, k))
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
