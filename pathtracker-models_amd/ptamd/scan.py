@@ -112,6 +112,8 @@ def gated_scan(x, h0=None, *, form="leaky", dim=1, gate_dim=2, lengths=None, wan
     Returns (y, h_last), for lstm (y, h_last, c_last): y in x's type and a
     gate's shape; h_last, f32, is y at each row's last step before its rounding
     (leaky: an empty row keeps h0; lstm: 0 there); c_last, f32, the last state.
+    Steps are composed before the state is known: one that becomes infinite may
+    be NaN in later steps.
     """
     return (_native or native()).gated_scan(x, h0, form, dim, gate_dim, lengths, want_seq)
 
