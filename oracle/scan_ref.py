@@ -20,8 +20,12 @@ than 2^-139.
 
 The error of a logistic value is (2 |x| + 8) u relative: |x| log2(e) is rounded
 once and its constant once (2 |x| u in the exponent), exp2 and the reciprocal
-are good to an ulp (2 u each), the sum to u.  tanh is good to 8 u absolute, its
-derivative to 16 u.  K = 24 covers the roundings of a step's own products and
+are good to an ulp (2 u each), the sum to u.  tanh is good to 8 u absolute and
+to 40 u relative: (1 - e) / (1 + e) with e = exp(-2|x|) is taken from 1/64 on at
+the least, where 1 - e >= 0.0307 makes at most 32.6 u of the ulp of e (u), the
+exponent adds 1.5 u (3 |x| u in e), the sum, the reciprocal and the products 5 u;
+below, 2x - 2x^2 + 4/3 x^3 leaves out 1/3 x^3 < 21.4 u of 1 - e and rounds four
+times.  tanh's derivative is good to 16 u.  K = 24 covers the roundings of a step's own products and
 of joining the pieces (at most 16 a chunk, of 4 steps or more each).
 """
 import torch
@@ -39,6 +43,11 @@ def _s(x):
 def _es(x):
     """Relative error of s(x) and s(-x); saturated values are exact."""
     return (2.0 * x.abs().clamp(max=104.0) + 8.0) * U
+
+
+def _et(th):
+    """Error of tanh where its value is at most th in size."""
+    return (40.0 * th.abs()).clamp(max=8.0) * U
 
 
 def walk(form, gates, h0=None, lengths=None, dy=None, dh=None, dc=None, backward=True):
@@ -63,7 +72,7 @@ def walk(form, gates, h0=None, lengths=None, dy=None, dh=None, dc=None, backward
         i, fg, pre, o = gates
         a, take, cand, show = _s(fg), _s(i), torch.tanh(pre), _s(o)
         ea = a * _es(fg)
-        eb = (take * cand).abs() * (_es(i) + 2 * U) + take * 8 * U
+        eb = (take * cand).abs() * (_es(i) + 2 * U) + take * _et(cand)
     put = take * cand
     a, put = torch.where(on, a, one), torch.where(on, put, zero)
     ea, eb = torch.where(on, ea, zero), torch.where(on, eb, zero)
@@ -88,7 +97,7 @@ def walk(form, gates, h0=None, lengths=None, dy=None, dh=None, dc=None, backward
     else:
         th = torch.tanh(st)
         y = show * th
-        ey = y.abs() * (_es(o) + 2 * U) + show * (est + 8 * U)
+        ey = y.abs() * (_es(o) + 2 * U) + show * (est + _et(th.abs() + est))
         h_last = torch.where(last, y, zero).sum(1)
         eh_last = torch.where(last, ey, zero).sum(1)
     val = dict(y=torch.where(on, y, zero), h=h_last, c=h)
@@ -134,10 +143,10 @@ def walk(form, gates, h0=None, lengths=None, dy=None, dh=None, dc=None, backward
     else:
         ki, kf, dt, ko = take * _s(-i), a * _s(-fg), 1.0 - cand * cand, show * _s(-o)
         dg = [G * cand * ki, G * bf * kf, G * take * dt, d * th * ko]
-        ed = [eG * cand.abs() * ki + G.abs() * ki * 8 * U + dg[0].abs() * (2 * _es(i) + 6 * U),
+        ed = [eG * cand.abs() * ki + G.abs() * ki * _et(cand) + dg[0].abs() * (2 * _es(i) + 6 * U),
               (eG * bf.abs() + G.abs() * ebf) * kf + dg[1].abs() * (2 * _es(fg) + 6 * U),
               eG * take * dt + G.abs() * take * 16 * U + dg[2].abs() * (_es(i) + 6 * U),
-              d.abs() * ko * (est + 8 * U) + dg[3].abs() * (2 * _es(o) + 6 * U)]
+              d.abs() * ko * (est + _et(th.abs() + est)) + dg[3].abs() * (2 * _es(o) + 6 * U)]
     val["dgates"] = [torch.where(on, v, zero) for v in dg]
     bnd["dgates"] = [torch.where(on, v + FG, zero) for v in ed]
     val["dh0"], bnd["dh0"] = g, eg
