@@ -202,6 +202,13 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Forward-mode derivatives: the kernels carry no tangents, and an input whose tangent
+// is passed over would look like a constant.
+void no_tangent(const Tensor& t, const char* op, PyObject* error) {
+  if (t._fw_grad(/*level=*/0).defined())
+    raise(error, std::string(op) + " has no forward-mode derivative: an input carries a tangent");
+}
+
 bool expanded(const Tensor& t) {
   for (int64_t k = 0; k < t.dim(); ++k)
     if (t.stride(k) == 0 && t.size(k) > 1) return true;
@@ -451,7 +458,7 @@ struct Taken {
   std::vector<int64_t> shape;
 };
 
-Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least) {
+Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, const char* op) {
   Taken t;
   if (THPVariable_Check(x.ptr())) {
     const Tensor v = THPVariable_Unpack(x.ptr());
@@ -482,6 +489,7 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least) {
                      ": dense float32, bfloat16 or float16");
     TORCH_CHECK_TYPE(v.scalar_type() == v0.scalar_type() && v.device() == v0.device(),
                      "the gates must have one type and one device");
+    no_tangent(v, op, scan_error_type);
   }
   if (!v0.is_cuda()) raise(scan_error_type, "the gated scan runs on a ROCm device only (no CPU fallback)");
   return t;
@@ -490,7 +498,8 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least) {
 py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::string& form_name, int64_t dim,
                      int64_t gate_dim, std::optional<Tensor> lengths, bool want_seq) {
   const Form form = form_of(form_name);
-  Taken t = take(x, form, gate_dim, 2);
+  if (h0) no_tangent(*h0, "gated_scan", scan_error_type);
+  Taken t = take(x, form, gate_dim, 2, "gated_scan");
   const int64_t nd = t.shape.size(), k = dim < 0 ? dim + nd : dim;
   TORCH_CHECK_VALUE(k >= 0 && k < nd, "dim ", dim, " is outside the tensor's ", nd, " dimensions");
   TORCH_CHECK_VALUE(k != t.gate_dim, "the gates cannot be stacked along the time dimension");
@@ -564,7 +573,8 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
 
 Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::string& form_name, int64_t gate_dim) {
   const Form form = form_of(form_name);
-  Taken t = take(x, form, gate_dim, 1);
+  no_tangent(state, "gated_scan_step", scan_error_type);
+  Taken t = take(x, form, gate_dim, 1, "gated_scan_step");
   TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat && state.device() == t.xs[0].device(),
                    "state must be a float32 tensor on the gates' device");
   TORCH_CHECK_VALUE(state.sizes() == at::IntArrayRef(t.shape), "state has shape ", state.sizes(), ", expected ",
@@ -634,6 +644,8 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   TORCH_CHECK_VALUE(code >= 0, "norm_type ", norm_type, ": 1, 2 or inf");
   const bool scale = max_norm >= 0.0;
   TORCH_CHECK_VALUE(!out || out->size() == grads.size(), out->size(), " outputs for ", grads.size(), " gradients");
+  for (const auto* list : {&grads, out ? &*out : &grads})
+    for (const auto& t : *list) no_tangent(t, "clipping", clip_error_type);
   check_tensors(grads, "gradients");
   if (out) {
     check_tensors(*out, "outputs");

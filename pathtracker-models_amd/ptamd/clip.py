@@ -90,7 +90,7 @@ def clip_grads(grads, max_norm, *, norm_type=2.0, out=None):
     norm before (f32, a device scalar; of no tensors: 0, on the CPU).
 
     grads: tensors of float32, bfloat16 or float16 (mixed, empty ones too) on
-      one device, sharing no memory with each other.
+      one device, sharing no memory with each other; no forward-mode tangents.
     out: None scales in place; else one tensor per gradient, of its shape and of
       its type or float32 (an optimizer's f32 buffers for 16-bit gradients).
     norm_type: 1, 2 or inf.

@@ -94,7 +94,8 @@ def native():
 
 
 def gated_scan(x, h0=None, *, form="leaky", dim=1, gate_dim=2, lengths=None, want_seq=True):
-    """The recurrence over a whole sequence, differentiable (once) in the gates and h0.
+    """The recurrence over a whole sequence, differentiable in the gates and h0 (once,
+    and backwards: an input with a forward-mode tangent is refused).
 
     x: the gates' pre-activations, stacked along ``gate_dim`` of one tensor
       ([B, T, G D] with the defaults; a Conv3d's [B, G C, T, H, W] has dim=2,
@@ -124,7 +125,7 @@ def gated_scan_step(x, state, *, form="leaky", gate_dim=1):
 
     x: the gates of this step stacked along ``gate_dim`` ([B, G D] with the
       default), or a sequence of G tensors; state: a gate's shape, any strides
-      that do not overlap.  No gradients: a step that needs them is a
-      ``gated_scan`` of one step.
+      that do not overlap.  No gradients and no tangents: a step that needs a
+      backward is a ``gated_scan`` of one step.
     """
     return (_native or native()).gated_scan_step(x, state, form, gate_dim)
