@@ -8,12 +8,14 @@
 // by path and called through their headers' functions.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -202,11 +204,26 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// Forward-mode derivatives: the kernels carry no tangents, and an input whose tangent
-// is passed over would look like a constant.
-void no_tangent(const Tensor& t, const char* op, PyObject* error) {
+// The operators are unknown to whatever records calls instead of making them: a trace
+// would hold the outputs' allocation alone and replay whatever stands in that memory.
+void not_recorded(const char* op, PyObject* error) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  bool recorded = torch::jit::tracer::isTracing();
+  for (auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+    recorded = recorded || TorchDispatchModeTLS::get_mode(k).has_value();
+  if (recorded) raise(error, std::string(op) + " cannot be traced");
+}
+
+// What the kernels cannot take an input for.  Forward-mode derivatives: they carry no
+// tangents, and an input whose tangent is passed over would look like a constant.
+// Tensors of a Python dispatch (traced, sharded, wrapping others): their address is
+// none, or not that of their values.
+void check_input(const Tensor& t, const char* op, PyObject* error) {
   if (t._fw_grad(/*level=*/0).defined())
     raise(error, std::string(op) + " has no forward-mode derivative: an input carries a tangent");
+  if (t.key_set().has(c10::DispatchKey::Python))
+    raise(error, std::string(op) + " takes plain tensors: a tensor with a dispatch of its own cannot be traced through it");
 }
 
 bool expanded(const Tensor& t) {
@@ -489,7 +506,7 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, cons
                      ": dense float32, bfloat16 or float16");
     TORCH_CHECK_TYPE(v.scalar_type() == v0.scalar_type() && v.device() == v0.device(),
                      "the gates must have one type and one device");
-    no_tangent(v, op, scan_error_type);
+    check_input(v, op, scan_error_type);
   }
   if (!v0.is_cuda()) raise(scan_error_type, "the gated scan runs on a ROCm device only (no CPU fallback)");
   return t;
@@ -498,7 +515,8 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, cons
 py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::string& form_name, int64_t dim,
                      int64_t gate_dim, std::optional<Tensor> lengths, bool want_seq) {
   const Form form = form_of(form_name);
-  if (h0) no_tangent(*h0, "gated_scan", scan_error_type);
+  not_recorded("gated_scan", scan_error_type);
+  if (h0) check_input(*h0, "gated_scan", scan_error_type);
   Taken t = take(x, form, gate_dim, 2, "gated_scan");
   const int64_t nd = t.shape.size(), k = dim < 0 ? dim + nd : dim;
   TORCH_CHECK_VALUE(k >= 0 && k < nd, "dim ", dim, " is outside the tensor's ", nd, " dimensions");
@@ -514,6 +532,7 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
     h = h0->to(at::kFloat).contiguous();
   }
   if (lengths) {
+    check_input(*lengths, "gated_scan", scan_error_type);
     TORCH_CHECK_VALUE(k != 0, "lengths need the batch in dimension 0, which is the time dimension here");
     TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == t.shape[0], "lengths has shape ", lengths->sizes(),
                       ", expected [", t.shape[0], "]");
@@ -573,7 +592,8 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
 
 Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::string& form_name, int64_t gate_dim) {
   const Form form = form_of(form_name);
-  no_tangent(state, "gated_scan_step", scan_error_type);
+  not_recorded("gated_scan_step", scan_error_type);
+  check_input(state, "gated_scan_step", scan_error_type);
   Taken t = take(x, form, gate_dim, 1, "gated_scan_step");
   TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat && state.device() == t.xs[0].device(),
                    "state must be a float32 tensor on the gates' device");
@@ -644,8 +664,9 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   TORCH_CHECK_VALUE(code >= 0, "norm_type ", norm_type, ": 1, 2 or inf");
   const bool scale = max_norm >= 0.0;
   TORCH_CHECK_VALUE(!out || out->size() == grads.size(), out->size(), " outputs for ", grads.size(), " gradients");
+  not_recorded("clipping", clip_error_type);
   for (const auto* list : {&grads, out ? &*out : &grads})
-    for (const auto& t : *list) no_tangent(t, "clipping", clip_error_type);
+    for (const auto& t : *list) check_input(t, "clipping", clip_error_type);
   check_tensors(grads, "gradients");
   if (out) {
     check_tensors(*out, "outputs");
