@@ -422,9 +422,9 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
                            const variable_list& grads) {
     Tensor dy = want_seq ? grads[0] : Tensor(), dh = grads[want_seq ? 1 : 0];
     Tensor dc = form.lstm() ? grads[want_seq ? 2 : 1] : Tensor();
-    if (dy.defined() && expanded(dy)) dy = dy.contiguous();      // (of a sum, a mean) no dense axis
-    if (dh.defined()) dh = dh.contiguous();
-    if (dc.defined()) dc = dc.contiguous();
+    if (dy.defined()) dy = (expanded(dy) ? dy.contiguous() : dy).resolve_neg();  // (of a sum, a mean) no dense axis
+    if (dh.defined()) dh = dh.contiguous().resolve_neg();
+    if (dc.defined()) dc = dc.contiguous().resolve_neg();
     Side x(xs, form.gates, gate_dim);
     Gates dxs;                           // stacked as x is, or one a gate
     if (gate_dim >= 0) dxs.push_back(at::empty_like(xs[0]));
@@ -508,6 +508,7 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, cons
                      "the gates must have one type and one device");
     check_input(v, op, scan_error_type);
   }
+  for (auto& v : t.xs) v = v.resolve_neg();
   if (!v0.is_cuda()) raise(scan_error_type, "the gated scan runs on a ROCm device only (no CPU fallback)");
   return t;
 }
@@ -529,7 +530,7 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
                       at::IntArrayRef(end));
     TORCH_CHECK_TYPE(h0->device() == device && h0->is_floating_point(),
                      "h0 must be a floating-point tensor on the gates' device");
-    h = h0->to(at::kFloat).contiguous();
+    h = h0->to(at::kFloat).contiguous().resolve_neg();
   }
   if (lengths) {
     check_input(*lengths, "gated_scan", scan_error_type);
@@ -539,7 +540,7 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
     TORCH_CHECK_TYPE(lengths->device() == device &&
                          at::isIntegralType(lengths->scalar_type(), /*includeBool=*/false),
                      "lengths must be an integer tensor on the gates' device");
-    len = lengths->to(at::kLong).contiguous();
+    len = lengths->to(at::kLong).contiguous().resolve_neg();
   }
   auto give = [&](const Tensor& y, const Tensor& hl, const Tensor& cl) -> py::tuple {
     py::object seq = want_seq ? py::cast(y) : py::none();
@@ -594,6 +595,7 @@ Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::stri
   const Form form = form_of(form_name);
   not_recorded("gated_scan_step", scan_error_type);
   check_input(state, "gated_scan_step", scan_error_type);
+  if (state.is_neg()) raise(scan_error_type, "state is a negated view: it cannot be updated in place");
   Taken t = take(x, form, gate_dim, 1, "gated_scan_step");
   TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat && state.device() == t.xs[0].device(),
                    "state must be a float32 tensor on the gates' device");
@@ -667,6 +669,10 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   not_recorded("clipping", clip_error_type);
   for (const auto* list : {&grads, out ? &*out : &grads})
     for (const auto& t : *list) check_input(t, "clipping", clip_error_type);
+  if (out)
+    for (size_t i = 0; i < grads.size(); ++i)
+      if ((*out)[i].is_neg() && !(*out)[i].is_same(grads[i]))
+        raise(clip_error_type, "an output is a negated view: it cannot be written");
   check_tensors(grads, "gradients");
   if (out) {
     check_tensors(*out, "outputs");
@@ -690,14 +696,15 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   for (size_t i = 0; i < grads.size(); ++i) {
     Tensor g = grads[i];
     const Tensor& o = out ? (*out)[i] : grads[i];
-    const bool place = scale && (!out || o.is_same(g) ||
-                                 (o.data_ptr() == g.data_ptr() && o.scalar_type() == g.scalar_type() &&
+    const bool place = scale && (!out || o.is_same(g) ||                 // (in place the sign does not matter)
+                                 (!g.is_neg() && o.data_ptr() == g.data_ptr() && o.scalar_type() == g.scalar_type() &&
                                   o.strides() == g.strides()));
     if (place && expanded(g))
       raise(clip_error_type,
             "a gradient's elements share memory (an expanded tensor): it cannot be clipped in place");
     const bool copied = !dense(g);
     if (copied) hold.push_back(g = g.contiguous());
+    if (!place && g.is_neg()) hold.push_back(g = g.resolve_neg());
     pt_clip_tensor& e = table[i];
     e.grad = g.data_ptr();
     e.n = g.numel();

@@ -1,0 +1,64 @@
+"""ptamd.scan and ptamd.clip on tensors whose memory does not hold their values as
+they are: views with the negative bit (x.conj().imag)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm device")
+    return torch.device("cuda:0")
+
+
+def _negated(v):
+    """The values of ``v`` in a view that holds their negatives."""
+    out = torch.complex(torch.zeros_like(v), -v).conj().imag
+    assert out.is_neg() and torch.equal(out, v)
+    return out
+
+
+@pytest.mark.parametrize("form,count", [("leaky", 2), ("lstm", 4)])
+def test_scan_of_negated_views(form, count):
+    from ptamd import scan
+    dev = _dev()
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(3, 40, count * 24, generator=g).to(dev)
+    h0 = torch.randn(3, 24, generator=g).to(dev)
+    dy, dh = torch.randn(3, 40, 24, generator=g).to(dev), torch.randn(3, 24, generator=g).to(dev)
+    ends = torch.tensor([40, 0, 17], device=dev)
+    outs = []
+    for neg in (lambda v: v, _negated):
+        for stacked in (True, False):
+            leaves = [v.clone().requires_grad_() for v in ([x] if stacked else x.chunk(count, 2))] + \
+                [h0.clone().requires_grad_()]
+            xs = [neg(v) for v in leaves[:-1]]
+            lengths = ends if neg is not _negated else torch._neg_view(-ends)
+            res = scan.gated_scan(xs[0] if stacked else xs, neg(leaves[-1]), form=form, lengths=lengths)
+            grads = torch.autograd.grad(res[:2], leaves, [neg(dy), neg(dh)])
+            with torch.no_grad():
+                again = scan.gated_scan(xs[0] if stacked else xs, neg(leaves[-1]), form=form, lengths=lengths)
+            outs.append([*(r.detach() for r in res), torch.cat(grads[:-1], 2), grads[-1], *again])
+            state = h0.clone()
+            one = [v[:, 3].detach() for v in xs]
+            outs[-1] += [scan.gated_scan_step(one[0] if stacked else one, state, form=form), state]
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+def test_clipping_of_negated_views():
+    from ptamd import clip
+    dev = _dev()
+    v = torch.randn(500, generator=torch.Generator().manual_seed(3)).to(dev)
+    for g in (_negated(v), _negated(torch.stack([v, v], 1))[:, 0]):
+        want = [torch.empty_like(v)]
+        norm = clip.clip_grads([v], 0.5, out=want)
+        got = [torch.empty_like(v)]
+        assert torch.equal(clip.clip_grads([g], 0.5, out=got), norm) and torch.equal(got[0], want[0])
+        assert torch.equal(clip.grad_norm([g]), norm)
+        assert torch.equal(clip.clip_grads([g], 0.5), norm) and torch.equal(g, want[0])     # in place
+    base = torch.complex(torch.zeros_like(v), -v)                     # its own memory as the output
+    g, o = base.conj().imag, base.imag
+    clip.clip_grads([g], 0.5, out=[o])
+    assert torch.equal(o, want[0])

@@ -70,3 +70,13 @@ def test_tensors_without_memory_of_their_own_are_refused():
             call()
     with pytest.raises(scan.PtScanError, match="plain tensors"):
         scan.gated_scan(torch.zeros(2, 5, 8), state)
+
+
+def test_writing_into_a_negated_view_is_refused():
+    """x.conj().imag holds the values' negatives: a kernel's store would land with the other sign."""
+    state = torch.zeros(2, 4, dtype=torch.complex64).conj().imag
+    assert state.is_neg() and state.dtype == torch.float32
+    with pytest.raises(scan.PtScanError, match="negated view"):
+        scan.gated_scan_step(torch.zeros(2, 8), state)
+    with pytest.raises(clip.PtClipError, match="negated view"):
+        clip.clip_grads([torch.zeros(2, 4)], 1.0, out=[state])
