@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <map>
 #include <optional>
 #include <string>
 #include <vector>
@@ -197,6 +198,72 @@ std::pair<uintptr_t, uintptr_t> span_of(const Tensor& t) {
 bool meet(const Tensor& a, const Tensor& b) {
   const auto x = span_of(a), y = span_of(b);
   return x.first < y.second && y.first < x.second;
+}
+
+// Whether an address difference lo .. hi plus step times x, x in its axis' range, over
+// all axes, can be 0.  Exact for strided tensors (views that interleave do not meet); it
+// gives up as "yes" where the axes nest so little that the search takes long.
+struct Axis {
+  int64_t step, lo, hi;
+};
+struct Reach {
+  std::vector<Axis> axes;                // the widest step first
+  std::vector<int64_t> least, most;      // of the axes from k on
+  int budget = 10000;
+
+  explicit Reach(std::vector<Axis> ax) : axes(std::move(ax)), least(axes.size() + 1), most(axes.size() + 1) {
+    std::sort(axes.begin(), axes.end(), [](const Axis& a, const Axis& b) { return a.step > b.step; });
+    for (size_t k = axes.size(); k-- > 0;) {
+      least[k] = least[k + 1] + axes[k].step * axes[k].lo;
+      most[k] = most[k + 1] + axes[k].step * axes[k].hi;
+    }
+  }
+  bool zero(int64_t lo, int64_t hi, size_t k = 0) {
+    if (k == axes.size()) return lo <= 0 && 0 <= hi;
+    const Axis& a = axes[k];
+    const int64_t from = std::max(a.lo, (int64_t)std::ceil((double)-(hi + most[k + 1]) / (double)a.step));
+    const int64_t to = std::min(a.hi, (int64_t)std::floor((double)-(lo + least[k + 1]) / (double)a.step));
+    for (int64_t x = from; x <= to; ++x)
+      if (--budget < 0 || zero(lo + a.step * x, hi + a.step * x, k + 1)) return true;
+    return false;
+  }
+};
+
+// Whether two tensors have a byte in common.
+bool intersect(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0 || !meet(a, b)) return false;
+  std::map<int64_t, Axis> ax;            // i steps of a and j of the same in b: i - j steps
+  auto axes_of = [&ax](const Tensor& t, int sign) {
+    for (int64_t k = 0; k < t.dim(); ++k) {
+      const int64_t st = t.stride(k) * (int64_t)t.element_size();
+      if (st == 0) continue;
+      Axis& x = ax.emplace(st, Axis{st, 0, 0}).first->second;
+      (sign > 0 ? x.hi : x.lo) += sign * (t.size(k) - 1);
+    }
+  };
+  axes_of(a, 1);
+  axes_of(b, -1);
+  std::vector<Axis> list;
+  for (const auto& [st, x] : ax) list.push_back(x);
+  const int64_t d = (int64_t)((intptr_t)a.data_ptr() - (intptr_t)b.data_ptr());
+  return Reach(list).zero(d - (int64_t)b.element_size() + 1, d + (int64_t)a.element_size() - 1);
+}
+
+// Whether two elements of one tensor share memory: places that differ, first in axis k.
+bool meets_itself(const Tensor& t) {
+  if (t.numel() == 0 || disjoint(t.sizes(), t.strides())) return false;
+  std::vector<Axis> ax;
+  for (int64_t k = 0; k < t.dim(); ++k)
+    if (t.size(k) > 1) {
+      if (t.stride(k) == 0) return true;
+      ax.push_back({t.stride(k), 1 - t.size(k), t.size(k) - 1});
+    }
+  for (; !ax.empty(); ax.pop_back()) {
+    auto some = ax;
+    some.back().lo = 1;
+    if (Reach(some).zero(0, 0)) return true;
+  }
+  return false;
 }
 
 // What autograd has to know of a tensor that a kernel wrote in place.
@@ -683,7 +750,7 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
       TORCH_CHECK_TYPE(o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat, "an output of type ",
                        o.scalar_type(), " for a gradient of type ", g.scalar_type());
       if (o.device() != g.device()) raise(clip_error_type, "outputs are not on the gradients' device");
-      if (!dense(o) && !disjoint(o.sizes(), o.strides()))
+      if (!dense(o) && meets_itself(o))
         raise(clip_error_type, "an output's elements share memory");
     }
   }
@@ -693,16 +760,19 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   std::vector<pt_clip_tensor> table(grads.size());
   std::vector<Tensor> hold;                              // dense copies
   std::vector<std::pair<Tensor, Tensor>> back;           // (tensor, dense copy): outputs to copy back
+  struct Aside { size_t i; Tensor t; bool written; };
+  std::vector<Aside> aside;                              // tensors that a copy stands for in the table
   for (size_t i = 0; i < grads.size(); ++i) {
     Tensor g = grads[i];
     const Tensor& o = out ? (*out)[i] : grads[i];
     const bool place = scale && (!out || o.is_same(g) ||                 // (in place the sign does not matter)
                                  (!g.is_neg() && o.data_ptr() == g.data_ptr() && o.scalar_type() == g.scalar_type() &&
                                   o.strides() == g.strides()));
-    if (place && expanded(g))
+    const bool copied = !dense(g);
+    if (place && copied && meets_itself(g))
       raise(clip_error_type,
             "a gradient's elements share memory (an expanded tensor): it cannot be clipped in place");
-    const bool copied = !dense(g);
+    if (copied) aside.push_back({i, g, place});
     if (copied) hold.push_back(g = g.contiguous());
     if (!place && g.is_neg()) hold.push_back(g = g.resolve_neg());
     pt_clip_tensor& e = table[i];
@@ -722,8 +792,19 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
       e.out = d.data_ptr();
       e.out_type = type_code(o.scalar_type());
       back.emplace_back(o, d);
+      aside.push_back({i, o, true});
     }
   }
+  // The library checks the memory that it is given.  What stands there for another
+  // tensor has to be as far apart as that tensor.
+  if (scale)
+    for (const Aside& s : aside)
+      for (size_t j = 0; j < grads.size(); ++j) {
+        if (j == s.i) continue;
+        const bool placed = !out || (*out)[j].is_same(grads[j]);
+        if (((s.written || placed) && intersect(s.t, grads[j])) || (out && intersect(s.t, (*out)[j])))
+          raise(clip_error_type, "a tensor that is written shares memory with another tensor of the call");
+      }
   const int64_t n = (int64_t)table.size();
   const size_t size = lib.clip_work(table.data(), n);
   if (!size) check_clip(PT_CLIP_ERR_ARG);
@@ -759,6 +840,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("gated_scan_step", torch::wrap_pybind_function(gated_scan_step));
   m.def("clip", torch::wrap_pybind_function(clip));
   m.def("fold", torch::wrap_pybind_function(py_fold));
+  m.def("intersect", torch::wrap_pybind_function(intersect));
+  m.def("meets_itself", torch::wrap_pybind_function(meets_itself));
   m.def("disjoint", [](const std::vector<int64_t>& sizes, const std::vector<int64_t>& strides) {
     return disjoint(sizes, strides);
   });

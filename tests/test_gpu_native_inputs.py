@@ -62,3 +62,40 @@ def test_clipping_of_negated_views():
     g, o = base.conj().imag, base.imag
     clip.clip_grads([g], 0.5, out=[o])
     assert torch.equal(o, want[0])
+
+
+def test_strided_tensors_that_share_memory_are_refused():
+    from ptamd import clip
+    dev = _dev()
+    base = torch.randn(40, 60, generator=torch.Generator().manual_seed(4)).to(dev)
+    kept = base.clone()
+    p = torch.nn.Parameter(torch.zeros(40, 30, device=dev))
+    p.grad = base[:, ::2]
+    free = torch.ones(40, 30, device=dev)
+    wide = torch.zeros(80, 60, device=dev)
+
+    def refused(*args, **kw):
+        with pytest.raises(clip.PtClipError, match="share"):
+            clip.clip_grads(*args, 1.0, **kw)
+        assert torch.equal(base, kept) and not wide.any()
+
+    with pytest.raises(clip.PtClipError, match="shares memory"):
+        clip.clip_grad_norm_([p, p], 1.0)
+    refused([base[:, ::2], base[:, ::2]])                                   # the same twice
+    refused([base[:, ::2], base[:, 2:4]])                                   # a column in both
+    refused([base[:, ::2], base.view(-1)[:70]])                             # a dense one over it
+    strided = [base[:, ::2], free]
+    refused(strided, out=[wide[::2, ::2], base[:, 2:32]])                   # an output on another gradient
+    refused(strided, out=[wide[::2, ::2], base.view(-1)[:1200].view(40, 30)])
+    refused(strided, out=[wide[::2, ::2], wide[::2, ::2]])                  # on another output
+    refused(strided, out=[wide[::2, ::2], wide[::2, :30]])
+    refused([free, kept[:, ::2]], out=[wide[::2, ::2], wide.view(-1)[:1200].view(40, 30)])
+    refused([base.as_strided((30, 4), (2, 1))])                             # elements of one gradient
+    # what interleaves, or is only read twice, goes on
+    norm = clip.clip_grads([base[:, ::2], base[:, 1::2]], 1.0)
+    want = kept.double().norm()
+    assert abs(float(norm) - float(want)) <= float(want) * 2.0 ** -23
+    torch.testing.assert_close(base, (kept.double() / (want + 1e-6)).float(), rtol=2.0 ** -22, atol=0)
+    out = [wide[::2, ::2], wide[1::2, 1::2]]
+    clip.clip_grads([kept[:, ::2], kept[:, ::2]], 1e9, out=out)
+    assert torch.equal(out[0], kept[:, ::2]) and torch.equal(out[1], kept[:, ::2])
