@@ -46,6 +46,9 @@ typedef struct pt_scan_desc {
     int64_t steps;      /* T, 1 to 2^30                                          */
     int64_t inner;      /* N, 1 to 2^29 - 1                                      */
 } pt_scan_desc;
+/* A call is one launch of fewer than 2^32 threads; what needs more is refused.  64
+ * columns of a row, or what is left of them, take 64 to 1024 threads, or, where there
+ * are few, 4 (leaky) or 8 (lstm) a step; an unaligned step takes one a column. */
 
 /* One sequence tensor: element strides over batch, channel and step.  The gates
  * of a call share theirs (as slices of one tensor do), and so do their

@@ -199,7 +199,7 @@ struct Where {
   int64_t state;             // this lane's column in [B][C][N]
   uint32_t off_c, off_n;     // channel in the group, position in the inner axis
 
-  __device__ __forceinline__ Where(const Args& a, uint32_t id) {    // the host keeps the grid below 2^31
+  __device__ __forceinline__ Where(const Args& a, uint32_t id) {    // the host keeps the grid below 2^26
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tile = id % (uint32_t)a.tiles;
@@ -1130,6 +1130,9 @@ int launch_t(int dtype, const Plan& p, const Args& a, int64_t blocks, bool bwd, 
   return launch_w<FORM, _Float16>(p, a, blocks, bwd, s);
 }
 
+// A launch counts its threads in 32 bits.
+bool fits_launch(double blocks, int threads) { return blocks * threads < 4294967296.0; }
+
 // The tensors of a call, checked.
 struct Tensors {
   const pt_scan_desc* d;
@@ -1175,8 +1178,9 @@ int run(const pt_scan_desc* d, const Plan& p, const Tensors& ts, Args& a, void* 
   a.segs = p.W ? 1 : (int)(bwd ? p.nchunks : (p.nchunks + 1) / 2);
   const int64_t tiles = (a.cg * a.N + 63) / 64;
   a.tiles = (int)tiles;
-  if ((double)tiles * (double)a.outer * (double)a.segs > 2147483647.0)
-    return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: too many columns for one launch");
+  const int threads = 64 * (p.W ? p.W : bwd ? CHAIN_BWD : CHAIN_FWD);
+  if (!fits_launch((double)tiles * (double)a.outer * (double)a.segs, threads))
+    return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: more columns and steps than one launch takes");
   if (!p.W) {
     if (!workspace || (uintptr_t)workspace % 16)
       return fail(PT_SCAN_ERR_ARG, "scan: this shape needs a workspace, aligned to 16 bytes");
@@ -1264,7 +1268,8 @@ int pt_scan_step(const pt_scan_desc* d, const pt_scan_view* x, const pt_scan_vie
   a.cols_all = d->batch * d->channels * d->inner;
   const int V = al ? 16 / ts.size : 1;
   const int64_t blocks = (a.cols_all / V + 255) / 256;
-  if (blocks > 2147483647) return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: too many columns for one launch");
+  if (!fits_launch((double)blocks, 256))
+    return fail(PT_SCAN_ERR_UNSUPPORTED, "scan: more columns than one launch takes");
   hipStream_t s = (hipStream_t)stream;
 #define PT_STEP(F, T, V_) hipLaunchKernelGGL((k_scan_step<F, T, V_>), dim3((unsigned)blocks), dim3(256), 0, s, a, sp, ss)
 #define PT_STEP_T(F)                                                                     \

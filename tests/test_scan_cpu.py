@@ -178,3 +178,23 @@ def test_fold_keeps_the_batch_apart():
     assert fold(y.shape, 0, (torch.empty(y.shape).stride(),), False)[:2] == (1, 1)
     # a step has neither: its columns may be cut anyhow
     assert fold((4, 6, 5, 8), -1, (x.select(1, 0).stride(),), -1)[0] == 24
+
+
+def test_more_threads_than_a_launch_takes_are_refused():
+    """Before anything is launched (a launch fails differently here, without a device)."""
+    lib = scan.load()
+    one = (scan.View * 4)(*[scan.View(4096, 0, 0, 0) for _ in range(4)])
+    ends = 4096
+
+    def rc(*desc):
+        d = scan.Desc(*desc)
+        out = [lib.pt_scan_forward(ctypes.byref(d), one, None, ends, None, None, None, None, 8192, None),
+               lib.pt_scan_backward(ctypes.byref(d), one, None, ends, None, None, None, 4096, one, None, 8192, None)]
+        return out, lib.pt_scan_last_error()
+
+    for desc in ((0, 1, 1, 1, 1 << 30, 1), (1, 1, 1, 1, 1 << 29, 64),          # chunks of one long row
+                 (0, 1, 1 << 24, 1, 100, 1), (1, 0, 1 << 26, 1, 4, 3)):        # rows, four waves and one
+        codes, word = rc(*desc)
+        assert codes == [2, 2] and b"launch takes" in word, (desc, codes, word)
+    d = scan.Desc(0, 0, 1 << 32, 1, 1, 1)
+    assert lib.pt_scan_step(ctypes.byref(d), one, one, one, None) == 2 and b"launch takes" in lib.pt_scan_last_error()
