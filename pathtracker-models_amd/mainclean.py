@@ -221,9 +221,10 @@ def main(argv=None):
             bucket.allreduce_mean()
             if args.clip_grad > 0:          # averaged gradients: every rank clips by the same factor
                 norm = clip_grad_norm_(model.parameters(), args.clip_grad)
-                train_log_dict['gradnorm'].append(norm.item())
             optimizer.step()
             optimizer.zero_grad()
+            if args.clip_grad > 0:          # (read behind the step: its launches do not wait for the backward)
+                train_log_dict['gradnorm'].append(norm.item())
             batch_time.update(time.perf_counter() - end)
             end = time.perf_counter()
             if idx % args.print_freq == 0 and main_rank:

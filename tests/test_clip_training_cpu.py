@@ -31,3 +31,51 @@ def test_convlstm_without_hidden_convolutions_keeps_the_parameters():
     assert frozen == {f"unit1.Wh{g}.weight" for g in "ifco"}
     with pytest.raises(RuntimeError, match="ROCm device"):
         cut(torch.zeros(1, 3, 8, 32, 32))
+
+
+class _Tiny(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.lin = torch.nn.Linear(3, 1)
+
+    def forward(self, x):
+        return self.lin(x.mean(dim=(2, 3, 4))), torch.ones(1)
+
+
+def _harness(tmp_path, monkeypatch, *flags):
+    """mainclean.py over synthetic clips with a CPU model and a CPU stand-in for the clipping."""
+    import mainclean
+    log = []
+
+    class Norm:
+        def item(self):
+            log.append("read")
+            return 1.5
+
+    def fake_clip(params, max_norm):
+        log.append(("clip", max_norm))
+        return Norm()
+
+    class Adam(torch.optim.SGD):
+        def __init__(self, params, lr, fused):
+            super().__init__(params, lr=lr)
+
+        def step(self):
+            log.append("step")
+            return super().step()
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    monkeypatch.setattr(mainclean.engine, "model_selector", lambda **kw: _Tiny())
+    monkeypatch.setattr(mainclean, "clip_grad_norm_", fake_clip)
+    monkeypatch.setattr(torch.optim, "Adam", Adam)
+    out = mainclean.main(["--model", "InT", "--name", "t", "--dist", "14", "--speed", "1", "--length", "4", "-b", "4",
+                          "--epochs", "1", "--data-root", str(tmp_path / "data"), "--synthetic", "16",
+                          "--results-root", str(tmp_path / "res"), "--max-iters", "2", *flags])
+    return log, out
+
+
+def test_the_norm_is_read_behind_the_step(tmp_path, monkeypatch):
+    """Its read waits for the whole backward: the step's launches go first."""
+    log, out = _harness(tmp_path, monkeypatch, "--clip-grad", "0.5")
+    assert log == [("clip", 0.5), "step", "read"] * 2
+    assert out["train"]["gradnorm"] == [1.5, 1.5]
