@@ -14,6 +14,14 @@ its own loop leaves uncalled):
 """
 import argparse
 
+
+def _max_norm(text):
+    value = float(text)
+    if not value >= 0.0:
+        raise argparse.ArgumentTypeError(f"{text}: a norm to clip to is not negative (0: no clipping)")
+    return value
+
+
 parser = argparse.ArgumentParser(description="PyTorch implementation of hGRU")
 
 parser.add_argument('--name', type=str, default="hgru")
@@ -61,7 +69,7 @@ parser.add_argument('--data-root', type=str, default=None)
 parser.add_argument('--synthetic', type=int, default=0)
 parser.add_argument('--results-root', type=str, default=None)
 parser.add_argument('--max-iters', type=int, default=0)
-parser.add_argument('--clip-grad', type=float, default=0.0, metavar='MAX',
+parser.add_argument('--clip-grad', type=_max_norm, default=0.0, metavar='MAX',
                     help='largest global gradient norm (L2, all parameters together, after the '
                          'averaging over the ranks); 0: no clipping (default)')
 parser.add_argument('--f32-input', default=False, action='store_true',

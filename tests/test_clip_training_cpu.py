@@ -79,3 +79,12 @@ def test_the_norm_is_read_behind_the_step(tmp_path, monkeypatch):
     log, out = _harness(tmp_path, monkeypatch, "--clip-grad", "0.5")
     assert log == [("clip", 0.5), "step", "read"] * 2
     assert out["train"]["gradnorm"] == [1.5, 1.5]
+
+
+@pytest.mark.parametrize("bad", ["-1", "nan", "-0.5", "x"])
+def test_a_norm_that_cannot_be_clipped_to_is_refused(bad, capsys):
+    """(-1 and nan would have trained without clipping, and said nothing)"""
+    with pytest.raises(SystemExit):
+        parser.parse_args(["--model", "InT", f"--clip-grad={bad}"])
+    assert "--clip-grad" in capsys.readouterr().err
+    assert parser.parse_args(["--model", "InT", "--clip-grad", "inf"]).clip_grad == float("inf")   # the norm alone
