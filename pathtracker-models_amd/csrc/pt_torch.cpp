@@ -615,8 +615,10 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
   };
   for (int64_t n : t.shape)
     if (n == 0) {                        // no step or no column: nothing to launch
-      const Tensor zero = at::zeros(end, t.xs[0].options().dtype(at::kFloat).requires_grad(false));
-      const Tensor c = h.defined() ? h.clone() : zero;
+      Tensor zero = at::zeros(end, t.xs[0].options().dtype(at::kFloat).requires_grad(false));
+      for (const auto& g : t.xs)         // a gradient to the gates has a place to go, as with steps
+        if (g.requires_grad()) zero = zero + g.sum(at::kFloat);
+      const Tensor c = !h.defined() ? zero : zero.requires_grad() ? h + zero : h.clone();
       Tensor y;
       if (want_seq)
         for (const auto& g : t.gate_dim >= 0 ? chunks(t.xs[0], form.gates, t.gate_dim) : t.xs)
