@@ -9,11 +9,13 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -23,6 +25,7 @@
 #include <map>
 #include <optional>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "pt_clip.h"
@@ -293,6 +296,32 @@ void check_input(const Tensor& t, const char* op, PyObject* error) {
     raise(error, std::string(op) + " takes plain tensors: a tensor with a dispatch of its own cannot be traced through it");
 }
 
+// Whether a backward that has come to `from` goes on to a node of the default stream:
+// the accumulator of a leaf that another graph, built there, keeps alive.  The engine
+// makes that stream wait for the present one, which no capture allows; in a captured
+// backward the process ends there.
+bool waits_on_default_stream(const torch::autograd::Node* from) {
+  const auto* exec = torch::autograd::get_current_graph_task_exec_info();   // null outside, empty: every node runs
+  std::vector<const torch::autograd::Node*> open{from};
+  std::unordered_set<const torch::autograd::Node*> seen{from};
+  while (!open.empty()) {
+    const auto* node = open.back();
+    open.pop_back();
+    for (const auto& edge : node->next_edges()) {
+      auto* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (exec && !exec->empty()) {
+        const auto it = exec->find(next);
+        if (it == exec->end() || !it->second.should_execute()) continue;
+      }
+      const auto stream = next->stream();
+      if (stream && stream->device_type() != c10::kCPU && stream->id() == 0) return true;
+      open.push_back(next);
+    }
+  }
+  return false;
+}
+
 bool expanded(const Tensor& t) {
   for (int64_t k = 0; k < t.dim(); ++k)
     if (t.stride(k) == 0 && t.size(k) > 1) return true;
@@ -469,6 +498,11 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
     const Tensor &lengths = saved[0], &h0 = saved[1], &states = saved[2];
     const Gates xs(saved.begin() + 3, saved.end());
     const c10::DeviceGuard guard(xs[0].device());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None &&
+        waits_on_default_stream(torch::autograd::get_current_node().get()))
+      raise(scan_error_type,
+            "gated_scan: a backward cannot be captured while a graph of the same leaves from the default stream "
+            "lives (a loss of an earlier pass, for one): release it first");
     variable_list out;
     {
       at::NoGradGuard no_grad;
@@ -842,6 +876,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("gated_scan_step", torch::wrap_pybind_function(gated_scan_step));
   m.def("clip", torch::wrap_pybind_function(clip));
   m.def("fold", torch::wrap_pybind_function(py_fold));
+  m.def("waits_on_default_stream",
+        [](const Tensor& t) { return t.grad_fn() && waits_on_default_stream(t.grad_fn().get()); });
   m.def("intersect", torch::wrap_pybind_function(intersect));
   m.def("meets_itself", torch::wrap_pybind_function(meets_itself));
   m.def("disjoint", [](const std::vector<int64_t>& sizes, const std::vector<int64_t>& strides) {

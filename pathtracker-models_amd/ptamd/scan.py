@@ -115,6 +115,8 @@ def gated_scan(x, h0=None, *, form="leaky", dim=1, gate_dim=2, lengths=None, wan
     (leaky: an empty row keeps h0; lstm: 0 there); c_last, f32, the last state.
     Steps are composed before the state is known: one that becomes infinite may
     be NaN in later steps.
+    Forward and backward can be captured into a graph; a captured backward of leaves
+    that a graph from the default stream still holds is refused.
     """
     return (_native or native()).gated_scan(x, h0, form, dim, gate_dim, lengths, want_seq)
 
