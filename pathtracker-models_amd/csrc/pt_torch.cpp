@@ -14,6 +14,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -274,27 +275,34 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// The operators are unknown to whatever records calls instead of making them: a trace
-// would hold the outputs' allocation alone and replay whatever stands in that memory.
-void not_recorded(const char* op, PyObject* error) {
-  using c10::impl::TorchDispatchModeKey;
-  using c10::impl::TorchDispatchModeTLS;
-  bool recorded = torch::jit::tracer::isTracing();
-  for (auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
-    recorded = recorded || TorchDispatchModeTLS::get_mode(k).has_value();
-  if (recorded) raise(error, std::string(op) + " cannot be traced");
-}
+// What a call cannot take, looked at once a call and once a tensor.
+struct Inputs {
+  const char* op;
+  PyObject* error;
+  bool tangents;                         // they live in a level alone (a view's is looked up in its base: 30 ns)
 
-// What the kernels cannot take an input for.  Forward-mode derivatives: they carry no
-// tangents, and an input whose tangent is passed over would look like a constant.
-// Tensors of a Python dispatch (traced, sharded, wrapping others): their address is
-// none, or not that of their values.
-void check_input(const Tensor& t, const char* op, PyObject* error) {
-  if (t._fw_grad(/*level=*/0).defined())
-    raise(error, std::string(op) + " has no forward-mode derivative: an input carries a tangent");
-  if (t.key_set().has(c10::DispatchKey::Python))
-    raise(error, std::string(op) + " takes plain tensors: a tensor with a dispatch of its own cannot be traced through it");
-}
+  // The operators are unknown to whatever records calls instead of making them: a trace
+  // would hold the outputs' allocation alone and replay whatever stands in that memory.
+  Inputs(const char* op, PyObject* error)
+      : op(op), error(error), tangents(torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    bool recorded = torch::jit::tracer::isTracing();
+    for (auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+      recorded = recorded || TorchDispatchModeTLS::get_mode(k).has_value();
+    if (recorded) raise(error, std::string(op) + " cannot be traced");
+  }
+  // Forward-mode derivatives: the kernels carry no tangents, and an input whose tangent is
+  // passed over would look like a constant.  Tensors of a Python dispatch (traced, sharded,
+  // wrapping others): their address is none, or not that of their values.
+  void check(const Tensor& t) const {
+    if (tangents && t._fw_grad(/*level=*/0).defined())
+      raise(error, std::string(op) + " has no forward-mode derivative: an input carries a tangent");
+    if (t.key_set().has(c10::DispatchKey::Python))
+      raise(error, std::string(op) +
+                       " takes plain tensors: a tensor with a dispatch of its own cannot be traced through it");
+  }
+};
 
 // Whether a backward that has come to `from` goes on to a node of the default stream:
 // the accumulator of a leaf that another graph, built there, keeps alive.  The engine
@@ -576,7 +584,7 @@ struct Taken {
   std::vector<int64_t> shape;
 };
 
-Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, const char* op) {
+Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, const Inputs& in) {
   Taken t;
   if (THPVariable_Check(x.ptr())) {
     const Tensor v = THPVariable_Unpack(x.ptr());
@@ -607,7 +615,7 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, cons
                      ": dense float32, bfloat16 or float16");
     TORCH_CHECK_TYPE(v.scalar_type() == v0.scalar_type() && v.device() == v0.device(),
                      "the gates must have one type and one device");
-    check_input(v, op, scan_error_type);
+    in.check(v);
   }
   for (auto& v : t.xs) v = v.resolve_neg();
   if (!v0.is_cuda()) raise(scan_error_type, "the gated scan runs on a ROCm device only (no CPU fallback)");
@@ -617,9 +625,9 @@ Taken take(const py::object& x, Form form, int64_t gate_dim, int64_t least, cons
 py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::string& form_name, int64_t dim,
                      int64_t gate_dim, std::optional<Tensor> lengths, bool want_seq) {
   const Form form = form_of(form_name);
-  not_recorded("gated_scan", scan_error_type);
-  if (h0) check_input(*h0, "gated_scan", scan_error_type);
-  Taken t = take(x, form, gate_dim, 2, "gated_scan");
+  const Inputs in("gated_scan", scan_error_type);
+  if (h0) in.check(*h0);
+  Taken t = take(x, form, gate_dim, 2, in);
   const int64_t nd = t.shape.size(), k = dim < 0 ? dim + nd : dim;
   TORCH_CHECK_VALUE(k >= 0 && k < nd, "dim ", dim, " is outside the tensor's ", nd, " dimensions");
   TORCH_CHECK_VALUE(k != t.gate_dim, "the gates cannot be stacked along the time dimension");
@@ -634,7 +642,7 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
     h = h0->to(at::kFloat).contiguous().resolve_neg();
   }
   if (lengths) {
-    check_input(*lengths, "gated_scan", scan_error_type);
+    in.check(*lengths);
     TORCH_CHECK_VALUE(k != 0, "lengths need the batch in dimension 0, which is the time dimension here");
     TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == t.shape[0], "lengths has shape ", lengths->sizes(),
                       ", expected [", t.shape[0], "]");
@@ -696,10 +704,10 @@ py::tuple gated_scan(const py::object& x, std::optional<Tensor> h0, const std::s
 
 Tensor gated_scan_step(const py::object& x, const Tensor& state, const std::string& form_name, int64_t gate_dim) {
   const Form form = form_of(form_name);
-  not_recorded("gated_scan_step", scan_error_type);
-  check_input(state, "gated_scan_step", scan_error_type);
+  const Inputs in("gated_scan_step", scan_error_type);
+  in.check(state);
   if (state.is_neg()) raise(scan_error_type, "state is a negated view: it cannot be updated in place");
-  Taken t = take(x, form, gate_dim, 1, "gated_scan_step");
+  Taken t = take(x, form, gate_dim, 1, in);
   TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat && state.device() == t.xs[0].device(),
                    "state must be a float32 tensor on the gates' device");
   TORCH_CHECK_VALUE(state.sizes() == at::IntArrayRef(t.shape), "state has shape ", state.sizes(), ", expected ",
@@ -769,9 +777,10 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   TORCH_CHECK_VALUE(code >= 0, "norm_type ", norm_type, ": 1, 2 or inf");
   const bool scale = max_norm >= 0.0;
   TORCH_CHECK_VALUE(!out || out->size() == grads.size(), out->size(), " outputs for ", grads.size(), " gradients");
-  not_recorded("clipping", clip_error_type);
-  for (const auto* list : {&grads, out ? &*out : &grads})
-    for (const auto& t : *list) check_input(t, "clipping", clip_error_type);
+  const Inputs in("clipping", clip_error_type);
+  for (const auto& t : grads) in.check(t);
+  if (out)
+    for (const auto& t : *out) in.check(t);
   if (out)
     for (size_t i = 0; i < grads.size(); ++i)
       if ((*out)[i].is_neg() && !(*out)[i].is_same(grads[i]))
