@@ -140,7 +140,7 @@ template <int P, typename T> __device__ __forceinline__ double chunk_norm(const 
   return acc;
 }
 
-// The partials.  Bound by memory: 335 million bf16 elements (671 MB) in 156 us, 4.3
+// The partials.  Bound by memory: 335 million bf16 elements (671 MB) in 153 us, 4.4
 // TB/s; 257 ragged tensors of three types (56 MB) in 16 us; 30 small ones in 5 us,
 // which is the launch.  512 or 2048 workgroups, chunks of 4096 or 16384: the same or
 // up to a tenth slower.
@@ -210,7 +210,7 @@ __device__ __forceinline__ void chunk_scale(const T* p, O* o, uint32_t n, double
   }
 }
 
-// The scaling: 335 million bf16 gradients into f32 (2.0 GB, two launches) in 375 us,
+// The scaling: 335 million bf16 gradients into f32 (2.0 GB, two launches) in 373 us,
 // 5.4 TB/s.  (With stores past the caches the whole call took 698 us instead of 567.)
 template <int P, bool OUT>
 __global__ __launch_bounds__(NT) void k_scale(Table<OUT> t, const double* part, int64_t parts, double max_norm,

@@ -150,7 +150,7 @@ template <bool ACC> __device__ __forceinline__ float tanh_d(float x, float& d) {
 
 // For 16-bit data: what s(x) is the reciprocal of, 1 + e^-x (infinite below -88, where
 // s(x) is then 0), and s(x) tanh(v) over one reciprocal.  A fifth fewer instructions a
-// step of the lstm's forward than with the functions above: 64 clips of 64 frames of
+// step of the lstm's forward than with the functions above (both without the series): 64 clips of 64 frames of
 // 25 x 32 x 32 162 to 145 us, 2 x 2048 x 6400 79 to 67.
 __device__ __forceinline__ float logistic_denom(float x) {
   return 1.f + __builtin_amdgcn_exp2f(x * in_scalar(-1.44269502f));
@@ -392,7 +392,8 @@ template <int FORM> __device__ __forceinline__ void last_states(const Args& a, c
 // finished.  Bound by memory where there are columns enough: leaky f32, 32 clips of 64 frames of 32 x 32 x 32 (805 MB) in
 // 159 us, 5.1 TB/s (a copy of 4 GiB reaches 4.8).  For 16 bits the arithmetic is
 // nearly as long as the loads: lstm bf16, 64 clips of 64 frames of 25 x 32 x 32
-// without y (629 MB), 145 us, 4.3 TB/s.  Of rows of unequal length the longest decides, where a
+// without y (629 MB), 138 us, 4.6 TB/s, and 172 in turn with its backward; lstm f32,
+// 32 of these clips with y (1049 MB), 226 us, 4.6 TB/s.  Of rows of unequal length the longest decides, where a
 // compute unit has one: leaky bf16 8 x 2048 x 2048, 68% of the steps live,
 // 40 us, 3.9 TB/s.
 template <int FORM, typename T, int W, int M>
@@ -626,8 +627,8 @@ template <int FORM> __device__ __forceinline__ float end_gradient(const Args& a,
 // Backward, a workgroup walking a column tile's whole row from its end.  Each
 // chunk is walked twice, both times from registers: forward from the kept state,
 // then back.  The shapes of the forward: leaky f32 (1342 MB) 261 us, 5.1 TB/s; lstm
-// bf16 (1468 MB) 334 us, 4.4 TB/s; leaky bf16 of unequal rows (271 MB) 78 us,
-// 3.5 TB/s.
+// bf16 (1468 MB) 331 us, 4.4 TB/s, and 346 in turn with its forward; lstm f32 with dy
+// (1887 MB) 375 us, 5.0 TB/s; leaky bf16 of unequal rows (271 MB) 78 us, 3.5 TB/s.
 template <int FORM, typename T, int W>
 __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
   constexpr int G = gates_of<FORM>(), L = back_steps<FORM>(), CH = W * L;
@@ -746,10 +747,13 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_bwd(Args a) {
 // nothing but the word is handed over.  NOT_YET is what no pair can be (its P
 // would be a NaN of a form that is never published).
 //
-// A chunk is loaded, joined and stored by one workgroup that does nothing else, so
-// that the memory waits for the joins at times: leaky bf16, 16384 steps of 2048
-// columns (201 MB), 57 us, 3.5 TB/s; lstm bf16, 2 rows of 8192 steps of 512
-// (84 and 151 MB), forward 30 us and backward 53 us, 2.8 and 2.8 TB/s.  Reading the
+// A chunk is loaded, joined and stored by one workgroup that does nothing else:
+// leaky bf16, 16384 steps of 2048 columns (201 MB), 57 us, 3.5 TB/s; lstm bf16, 2 rows
+// of 8192 steps of 512 (84 and 151 MB), forward 31 us and backward 55 us, 2.7 TB/s
+// both; the same in f32 51 and 73 us, 3.3 and 4.1 TB/s.  Twice the bytes do not take
+// twice the time: part of it is a chunk's own, whatever it holds.  Waves wait 58 to 63 %
+// of their cycles and issue vector instructions in about a tenth; the counters do not
+// tell the wait for a join from that for loads.  Reading the
 // sequence twice instead (every chunk's pair, then the walk) took, at 16384 steps
 // of 2048 columns, for leaky f32 128 us and in the backward 194, against 95 and
 // 132 here; for lstm bf16 128 and 248, against 113 and 193.  A workgroup that
@@ -1053,6 +1057,17 @@ struct Plan {
 //                 waves.  (4096 steps of leaky bf16, forward and backward: 64
 //                 tiles 42 and 47 us, 66 and 107 with 16 waves; 128 tiles 66 and
 //                 93, 67 and 136; 256 tiles 127 and 176, 95 and 147.)
+// The limits were found with leaky bf16.  The other kinds at 2048 steps, forward /
+// backward in us (what the rule takes stands first):
+//            leaky f32                    lstm bf16                     lstm f32
+//   128  chain 42/72, 16: 37/89      chain 50/106, 16: 68/156     chain 99/126, 16: 110/174
+//   180  16: 54/101, chain 62/98     16: 68/159, chain 67/147     16: 121/190, chain 136/175
+//   256  16: 82/136, 8: 79/129       16: 80/169, 8: 82/172        16: 146/243, 8: 144/229
+//   300  8: 120/199, chain 103/153   8: 127/256, chain 113/239    8: 232/383, chain 215/280
+//   512  8: 166/275, 4: 166/266      8: 148/276, 4: 159/337       8: 287/510, 4: 288/471
+//   700  4: 235/387, 8: 231/380      4: 214/428, 8: 207/378       4: 421/729, 8: 414/719
+// Just above 256 tiles the chain is 7 to 27 % faster for them, at 700 8 waves for lstm
+// bf16's backward by 12 %.
 // Up to 4 L steps fit a chunk of 4 waves, up to L steps one wave.
 Plan plan_of(const pt_scan_desc* d) {
   Plan p;
