@@ -767,6 +767,41 @@ void check_tensors(const std::vector<Tensor>& ts, const char* what) {
   }
 }
 
+// The library checks the memory that it is given.  Where a copy stands for a gradient or an
+// output there (`aside`), the tensors themselves have to be apart from all others.
+void check_aside(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out,
+                 const std::vector<size_t>& aside) {
+  struct Span {
+    uintptr_t lo, hi, before;            // before: the furthest end of the spans in front
+    size_t i;
+    const Tensor* t;
+    bool written;
+  };
+  std::vector<Span> all;
+  auto add = [&all](const Tensor& t, size_t i, bool written) {
+    if (t.numel() == 0) return;
+    const auto [lo, hi] = span_of(t);
+    all.push_back({lo, hi, 0, i, &t, written});
+  };
+  for (size_t i = 0; i < grads.size(); ++i) {
+    add(grads[i], i, !out);
+    if (out) add((*out)[i], i, true);
+  }
+  std::sort(all.begin(), all.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  for (size_t k = 1; k < all.size(); ++k) all[k].before = std::max(all[k - 1].before, all[k - 1].hi);
+  auto apart = [](const Span& a, const Span& b) {
+    if (a.i != b.i && (a.written || b.written) && intersect(*a.t, *b.t))
+      raise(clip_error_type, "a tensor that is written shares memory with another tensor of the call");
+  };
+  std::vector<bool> is_aside(grads.size());
+  for (size_t i : aside) is_aside[i] = true;
+  for (size_t k = 0; k < all.size(); ++k) {
+    if (!is_aside[all[k].i]) continue;
+    for (size_t j = k + 1; j < all.size() && all[j].lo < all[k].hi; ++j) apart(all[k], all[j]);
+    for (size_t j = k; j > 0 && all[j].before > all[k].lo; --j) apart(all[k], all[j - 1]);
+  }
+}
+
 // The norm of `grads`; with max_norm >= 0 they are clipped, into `out` or in place.
 Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
             const std::optional<std::vector<Tensor>>& out) {
@@ -805,21 +840,21 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
   std::vector<pt_clip_tensor> table(grads.size());
   std::vector<Tensor> hold;                              // dense copies
   std::vector<std::pair<Tensor, Tensor>> back;           // (tensor, dense copy): outputs to copy back
-  struct Aside { size_t i; Tensor t; bool written; };
-  std::vector<Aside> aside;                              // tensors that a copy stands for in the table
+  std::vector<size_t> aside;                             // where a copy stands for a tensor in the table
   for (size_t i = 0; i < grads.size(); ++i) {
     Tensor g = grads[i];
     const Tensor& o = out ? (*out)[i] : grads[i];
     const bool place = scale && (!out || o.is_same(g) ||                 // (in place the sign does not matter)
                                  (!g.is_neg() && o.data_ptr() == g.data_ptr() && o.scalar_type() == g.scalar_type() &&
                                   o.strides() == g.strides()));
-    const bool copied = !dense(g);
-    if (place && copied && meets_itself(g))
+    const bool strided = !dense(g), copied = strided || (!place && g.is_neg());
+    if (place && strided && meets_itself(g))
       raise(clip_error_type,
             "a gradient's elements share memory (an expanded tensor): it cannot be clipped in place");
-    if (copied) aside.push_back({i, g, place});
-    if (copied) hold.push_back(g = g.contiguous());
-    if (!place && g.is_neg()) hold.push_back(g = g.resolve_neg());
+    if (scale && copied) aside.push_back(i);
+    if (strided) g = g.contiguous();
+    if (!place) g = g.resolve_neg();
+    if (copied) hold.push_back(g);
     pt_clip_tensor& e = table[i];
     e.grad = g.data_ptr();
     e.n = g.numel();
@@ -837,19 +872,10 @@ Tensor clip(const std::vector<Tensor>& grads, double norm_type, double max_norm,
       e.out = d.data_ptr();
       e.out_type = type_code(o.scalar_type());
       back.emplace_back(o, d);
-      aside.push_back({i, o, true});
+      if (!copied) aside.push_back(i);
     }
   }
-  // The library checks the memory that it is given.  What stands there for another
-  // tensor has to be as far apart as that tensor.
-  if (scale)
-    for (const Aside& s : aside)
-      for (size_t j = 0; j < grads.size(); ++j) {
-        if (j == s.i) continue;
-        const bool placed = !out || (*out)[j].is_same(grads[j]);
-        if (((s.written || placed) && intersect(s.t, grads[j])) || (out && intersect(s.t, (*out)[j])))
-          raise(clip_error_type, "a tensor that is written shares memory with another tensor of the call");
-      }
+  if (!aside.empty()) check_aside(grads, out, aside);
   const int64_t n = (int64_t)table.size();
   const size_t size = lib.clip_work(table.data(), n);
   if (!size) check_clip(PT_CLIP_ERR_ARG);

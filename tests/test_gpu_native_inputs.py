@@ -99,3 +99,29 @@ def test_strided_tensors_that_share_memory_are_refused():
     out = [wide[::2, ::2], wide[1::2, 1::2]]
     clip.clip_grads([kept[:, ::2], kept[:, ::2]], 1e9, out=out)
     assert torch.equal(out[0], kept[:, ::2]) and torch.equal(out[1], kept[:, ::2])
+
+
+def test_one_overlap_among_many_strided_gradients():
+    """Wherever it stands in the list and in memory."""
+    from ptamd import clip
+    dev = _dev()
+    flat = torch.ones(300, 40, 10, device=dev)
+    grads = [flat[k, :, ::2] for k in range(300)]
+    assert abs(float(clip.clip_grads(grads, 1e9)) - 60_000 ** 0.5) < 1e-4
+    for k in (0, 123, 299):
+        other = flat[k, 5:9, 4:7]
+        for at in (0, 77, 300):
+            with pytest.raises(clip.PtClipError, match="share"):
+                clip.clip_grads(grads[:at] + [other] + grads[at:], 1.0)
+    wide = flat[:, 0].t()                                    # over all of them
+    with pytest.raises(clip.PtClipError, match="share"):
+        clip.clip_grads(grads[7:9] + [wide], 1.0)
+    assert bool((flat == 1).all())
+
+
+def test_an_output_on_a_negated_gradient_is_refused():
+    from ptamd import clip
+    v, w = torch.ones(60, device=_dev()), torch.ones(60, device=_dev())
+    with pytest.raises(clip.PtClipError, match="share"):
+        clip.clip_grads([torch._neg_view(v), w], 1.0, out=[torch.empty_like(v), v])
+    assert bool((v == 1).all())
