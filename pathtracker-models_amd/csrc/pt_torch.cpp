@@ -300,7 +300,7 @@ struct Inputs {
       raise(error, std::string(op) + " has no forward-mode derivative: an input carries a tangent");
     if (t.key_set().has(c10::DispatchKey::Python))
       raise(error, std::string(op) +
-                       " takes plain tensors: a tensor with a dispatch of its own cannot be traced through it");
+                       " takes plain tensors: one with a Python dispatch has no memory that a kernel could read");
   }
 };
 
@@ -511,6 +511,9 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
       raise(scan_error_type,
             "gated_scan: a backward cannot be captured while a graph of the same leaves from the default stream "
             "lives (a loss of an earlier pass, for one): release it first");
+    const Inputs in("gated_scan", scan_error_type);
+    for (const auto& g : grads)          // (of no address they would pass for absent)
+      if (g.defined()) in.check(g);
     variable_list out;
     {
       at::NoGradGuard no_grad;

@@ -125,3 +125,39 @@ def test_an_output_on_a_negated_gradient_is_refused():
     with pytest.raises(clip.PtClipError, match="share"):
         clip.clip_grads([torch._neg_view(v), w], 1.0, out=[torch.empty_like(v), v])
     assert bool((v == 1).all())
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor that holds another and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        out = torch.Tensor._make_wrapper_subclass(cls, inner.shape, strides=inner.stride(), dtype=inner.dtype,
+                                                  device=inner.device)
+        out.inner = inner
+        return out
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        def plain(v):
+            return v.inner if isinstance(v, cls) else v
+        return func(*torch.utils._pytree.tree_map(plain, args), **torch.utils._pytree.tree_map(plain, kwargs or {}))
+
+
+def test_gradients_that_are_no_plain_tensors_are_refused():
+    from ptamd import scan
+    import torch.autograd.forward_ad as fwAD
+    dev = _dev()
+    x = torch.randn(2, 30, 16, device=dev, requires_grad=True)
+    d = torch.randn(2, 30, 8, device=dev)
+    y, h = scan.gated_scan(x)
+    with pytest.raises(RuntimeError, match="plain tensors"):
+        torch.autograd.grad(y, x, _Wrapped(d), retain_graph=True)
+    with pytest.raises(RuntimeError, match="plain tensors"):
+        torch.autograd.grad([y, h], x, [d, _Wrapped(d[:, 0].contiguous())], retain_graph=True)
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        torch.autograd.grad(y, x, fwAD.make_dual(d, torch.ones_like(d)), retain_graph=True)
+    with pytest.raises(scan.PtScanError, match="plain tensors"):
+        scan.gated_scan(_Wrapped(x.detach()))
+    want, = torch.autograd.grad(y, x, d, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, x, d)[0], want) and bool(want.any())
